@@ -51,6 +51,20 @@ EXPORTED_LAYERS = (
     "ebr_descent_step_scratch_floats",
 )
 
+# include/ebr_tokens.h: the operators driven by integer ids.
+EXPORTED_TOKENS = (
+    "ebr_scaled_embedding",
+    "ebr_scaled_embedding_grad",
+    "ebr_scaled_embedding_grad_scratch_bytes",
+    "ebr_expert_route",
+    "ebr_expert_route_scratch_bytes",
+    "ebr_expert_scatter",
+    "ebr_expert_combine",
+    "ebr_topk_distill",
+    "ebr_topk_distill_grad",
+)
+INT32, INT64 = 0, 1  # ebr_id_type
+
 
 class Operand(ctypes.Structure):
     """``ebr_operand``: a strided [B, H, N, D] operand (strides in elements, unit head-dim stride)."""
@@ -121,6 +135,19 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.ebr_descent_step_scratch_floats.restype = sz
     for name in EXPORTED_LAYERS[:-1]:
         getattr(lib, name).restype = ctypes.c_int
+    it = ctypes.c_int
+    lib.ebr_scaled_embedding.argtypes = [it, it, it, i64, i64, i64, dbl, vp, vp, i64, vp, vp]
+    lib.ebr_scaled_embedding_grad.argtypes = [it, it, it, i64, i64, i64, dbl, vp, vp, i64, vp, vp, sz, vp]
+    lib.ebr_scaled_embedding_grad_scratch_bytes.argtypes = [i64, i64, i64]
+    lib.ebr_expert_route.argtypes = [it, i64, i64, i64, i64, vp, vp, vp, vp, vp, sz, vp]
+    lib.ebr_expert_route_scratch_bytes.argtypes = [i64, i64, i64]
+    lib.ebr_expert_scatter.argtypes = [it, it, i64, i64, i64, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp]
+    lib.ebr_expert_combine.argtypes = [it, it, i64, i64, i64, vp, i64, vp, vp, vp, vp]
+    lib.ebr_topk_distill.argtypes = [it, it, it, i64, i64, i64, dbl, dbl, vp, i64, vp, vp, vp, vp, vp, vp, vp, vp]
+    lib.ebr_topk_distill_grad.argtypes = [it, it, it, i64, i64, i64, dbl, dbl, vp, i64, vp, vp, vp, vp, vp, i64, it,
+                                          vp, vp]  # fmt: skip
+    for name in EXPORTED_TOKENS:
+        getattr(lib, name).restype = sz if name.endswith("_bytes") else ctypes.c_int
 
 
 def lib() -> ctypes.CDLL:

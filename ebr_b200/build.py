@@ -41,7 +41,8 @@ def _nvcc() -> str:
 
 
 def sources() -> list[Path]:
-    return sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + [ROOT / "include" / "ebr_attn.h", ROOT / "include" / "ebr_layers.h"]
+    headers = [ROOT / "include" / name for name in ("ebr_attn.h", "ebr_layers.h", "ebr_tokens.h")]
+    return sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + headers
 
 
 def up_to_date() -> bool:

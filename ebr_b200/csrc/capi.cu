@@ -869,3 +869,6 @@ uint64_t ebr_attn_launch_count(void) { return g_launch_count.load(); }
 
 // The fused kernels on either side of the attention (include/ebr_layers.h).
 #include "layers_capi.cuh"
+
+// The operators driven by integer ids (include/ebr_tokens.h).
+#include "tokens_capi.cuh"

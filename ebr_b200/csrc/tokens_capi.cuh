@@ -1,0 +1,571 @@
+// tokens_capi.cuh: the C ABI of include/ebr_tokens.h (included at the end of capi.cu, after layers_capi.cuh, whose
+// dtype and alignment helpers it uses). Validates arguments, picks the access width and launch shape, and launches the
+// kernels of key_sort.cuh, embedding.cuh, experts.cuh and distill.cuh on the caller's stream.
+#pragma once
+
+#include "../../include/ebr_tokens.h"
+#include "distill.cuh"
+#include "embedding.cuh"
+#include "experts.cuh"
+#include "key_sort.cuh"
+
+namespace {
+
+using ebr::keysort::ClusterSort;
+using ebr::keysort::GridSort;
+using ebr::keysort::IdSource;
+
+constexpr int64_t kMaxSortKeys = int64_t{1} << 30;
+constexpr int kMaxExperts = 1 << ebr::keysort::kMaxDigitBits;
+
+int check_id_type(int id_type) {
+  return id_type == EBR_INT32 || id_type == EBR_INT64 ? EBR_OK : set_error(EBR_ERR_DTYPE, "ids must be int32 or int64%s%s");
+}
+
+size_t round16(size_t b) { return (b + 15) & ~size_t{15}; }
+
+// Run fn(tag of A, tag of B) for two I/O types.
+template <typename Fn>
+int with_types(int a, int b, Fn&& fn) {
+  return with_type(a, [&](auto* ta) -> int {
+    if constexpr (std::is_same_v<std::remove_pointer_t<decltype(ta)>, double>) {
+      return set_error(EBR_ERR_DTYPE, "float64 is not a type of this operator%s%s");
+    } else {
+      return with_type(b, [&](auto* tb) -> int {
+        if constexpr (std::is_same_v<std::remove_pointer_t<decltype(tb)>, double>)
+          return set_error(EBR_ERR_DTYPE, "float64 is not a type of this operator%s%s");
+        else
+          return fn(ta, tb);
+      });
+    }
+  });
+}
+
+// Run fn(integral constant V) with the widest V of {8, 4, 2, 1} (at most `most`) for which rows of C elements and the
+// given row strides and pointers keep every access of V elements of `size` bytes (16 at most) aligned.
+struct Rows {
+  const void* p;
+  int64_t stride;
+  int size;
+};
+
+int access_width(int most, int64_t C, std::initializer_list<Rows> rows) {
+  int v = most;
+  for (; v > 1; v /= 2) {
+    bool ok = C % v == 0;
+    for (const Rows& r : rows) {
+      const int64_t bytes = std::min<int64_t>(16, static_cast<int64_t>(v) * r.size);
+      ok = ok && reinterpret_cast<uintptr_t>(r.p) % bytes == 0 && (r.stride * r.size) % bytes == 0;
+    }
+    if (ok) break;
+  }
+  return v;
+}
+
+template <typename Fn>
+int with_width(int v, Fn&& fn) {
+  switch (v) {
+    case 8: return fn(std::integral_constant<int, 8>{});
+    case 4: return fn(std::integral_constant<int, 4>{});
+    case 2: return fn(std::integral_constant<int, 2>{});
+    default: return fn(std::integral_constant<int, 1>{});
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ sort
+
+// Keys that one cluster of 16 CTAs ranks in registers.
+constexpr int64_t kClusterKeys = 16 * int64_t{ebr::keysort::kSortThreads} * 16;
+
+int digit_passes(int64_t range) {  // keys in [0, range]
+  int bits = 1;
+  while ((int64_t{1} << bits) <= range) ++bits;
+  return (bits + ebr::keysort::kMaxDigitBits - 1) / ebr::keysort::kMaxDigitBits;
+}
+
+int digit_bits(int64_t range, int passes) {
+  int bits = 1;
+  while ((int64_t{1} << bits) <= range) ++bits;
+  return (bits + passes - 1) / passes;
+}
+
+int64_t sort_tiles(int64_t n) { return (n + ebr::keysort::kTile - 1) / ebr::keysort::kTile; }
+
+// Scratch of a sort: two (key, position) arrays where there is output, and the whole-grid path's counts.
+size_t sort_scratch(int64_t n, int64_t digits, int passes, bool route) {
+  size_t b = 0;
+  if (!route) b += (passes > 1 ? 4 : 2) * round16(static_cast<size_t>(n) * 4);
+  if (n > kClusterKeys) b += round16(static_cast<size_t>(digits) * sort_tiles(n) * 4) + round16(digits * 4);
+  return b;
+}
+
+template <int kItems>
+int launch_cluster_sort(int device, const ClusterSort& a, int ctas, int bits, int fill_clusters, cudaStream_t st) {
+  auto* kernel = ebr::keysort::cluster_sort_kernel<kItems>;
+  static std::atomic<bool> ready[kMaxDevices];
+  if (device >= kMaxDevices || !ready[device].load()) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               static_cast<int>(ebr::keysort::cluster_sort_smem(ebr::keysort::kMaxDigitBits)));
+    if (e != cudaSuccess) return cuda_error(e, "cluster sort attributes");
+    if (device < kMaxDevices) ready[device].store(true);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas * (1 + fill_clusters)));
+  cfg.blockDim = dim3(ebr::keysort::kSortThreads);
+  cfg.dynamicSmemBytes = ebr::keysort::cluster_sort_smem(bits);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim = {static_cast<unsigned>(ctas), 1, 1};
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+  if (e != cudaSuccess) return cuda_error(e, "cluster sort");
+  return check_launch("cluster sort");
+}
+
+// Sort n keys of [0, range]; digits: of one pass. For a route (route.row_of set) there is one pass, else the sorted keys
+// and positions are at *key / *order in the scratch. `fill` bytes are zeroed beside or before the sort.
+int run_sort(int device, IdSource src, int64_t n, int passes, int bits, const ebr::keysort::RouteOut& route,
+             void* scratch, int** key, int** order, void* fill, int64_t fill_bytes, cudaStream_t st) {
+  char* at = static_cast<char*>(scratch);
+  auto take = [&](size_t bytes) {
+    char* p = at;
+    at += round16(bytes);
+    return reinterpret_cast<int*>(p);
+  };
+  ebr::keysort::Pass pass[3] = {};
+  const bool is_route = route.row_of != nullptr;
+  if (!is_route) {
+    int* buf[4] = {take(n * 4), take(n * 4), nullptr, nullptr};
+    if (passes > 1) {
+      buf[2] = take(n * 4);
+      buf[3] = take(n * 4);
+    }
+    for (int p = 0; p < passes; ++p) {
+      const int to = (passes - 1 - p) % 2;  // the last pass writes the first pair
+      pass[p].key_in = p ? buf[2 * (1 - to)] : nullptr;
+      pass[p].idx_in = p ? buf[2 * (1 - to) + 1] : nullptr;
+      pass[p].key_out = buf[2 * to];
+      pass[p].idx_out = buf[2 * to + 1];
+      pass[p].shift = p * bits;
+      pass[p].bits = bits;
+    }
+    *key = buf[0];
+    *order = buf[1];
+  } else {
+    pass[0].bits = bits;
+  }
+  if (n <= kClusterKeys) {
+    ClusterSort a = {};
+    a.src = src;
+    a.n = n;
+    a.passes = passes;
+    for (int p = 0; p < 3; ++p) a.pass[p] = pass[p];
+    a.route = route;
+    a.fill = fill;
+    a.fill_bytes = fill_bytes;
+    int ctas = 1;
+    while (ctas < 16 && static_cast<int64_t>(ctas) * ebr::keysort::kSortThreads < n) ctas *= 2;
+    const int64_t per_thread = ((n + ctas - 1) / ctas + ebr::keysort::kSortThreads - 1) / ebr::keysort::kSortThreads;
+    // zeroing CTAs: one for 64 KB, whole clusters, at most what fills the other SMs once
+    int64_t fill_ctas = fill ? std::min<int64_t>((fill_bytes + 65535) / 65536, sm_count(device)) : 0;
+    if (fill && fill_ctas == 0) fill_ctas = 1;
+    const int fill_clusters = static_cast<int>((fill_ctas + ctas - 1) / ctas);
+    if (per_thread <= 1) return launch_cluster_sort<1>(device, a, ctas, bits, fill_clusters, st);
+    if (per_thread <= 2) return launch_cluster_sort<2>(device, a, ctas, bits, fill_clusters, st);
+    if (per_thread <= 4) return launch_cluster_sort<4>(device, a, ctas, bits, fill_clusters, st);
+    if (per_thread <= 8) return launch_cluster_sort<8>(device, a, ctas, bits, fill_clusters, st);
+    return launch_cluster_sort<16>(device, a, ctas, bits, fill_clusters, st);
+  }
+  if (fill && fill_bytes) {
+    const cudaError_t e = cudaMemsetAsync(fill, 0, static_cast<size_t>(fill_bytes), st);
+    if (e != cudaSuccess) return cuda_error(e, "zeroing");
+  }
+  GridSort g = {};
+  g.src = src;
+  g.n = n;
+  g.digits = is_route ? route.experts : 1 << bits;
+  g.tiles = static_cast<int>(sort_tiles(n));
+  g.counts = take(static_cast<size_t>(g.digits) * g.tiles * 4);
+  g.totals = take(static_cast<size_t>(g.digits) * 4);
+  g.route = route;
+  const size_t smem = ebr::keysort::grid_place_smem(g.digits);
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(ebr::keysort::grid_place_kernel,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return cuda_error(e, "sort attributes");
+  }
+  for (int p = 0; p < passes; ++p) {
+    g.pass = pass[p];
+    ebr::keysort::grid_count_kernel<<<g.tiles, ebr::keysort::kSortThreads, g.digits * 4, st>>>(g);
+    int rc = check_launch("sort count");
+    if (rc != EBR_OK) return rc;
+    ebr::keysort::grid_scan_kernel<<<g.digits, ebr::keysort::kSortThreads, 0, st>>>(g);
+    if ((rc = check_launch("sort scan")) != EBR_OK) return rc;
+    ebr::keysort::grid_place_kernel<<<g.tiles, ebr::keysort::kSortThreads, smem, st>>>(g);
+    if ((rc = check_launch("sort place")) != EBR_OK) return rc;
+  }
+  return EBR_OK;
+}
+
+// ------------------------------------------------------------------------------------------------ embedding
+
+int check_embedding(int id_type, int64_t n, int64_t V, int64_t C, int64_t stride) {
+  int rc = check_id_type(id_type);
+  if (rc != EBR_OK) return rc;
+  if (n < 0 || V < 1 || C < 1) return set_error(EBR_ERR_SHAPE, "embedding: bad sizes%s%s");
+  if (n >= kMaxSortKeys || V >= kMaxSortKeys || C > (1 << 24))
+    return set_error(EBR_ERR_SHAPE, "embedding: size too large%s%s");
+  if (stride < 0) return set_error(EBR_ERR_STRIDE, "embedding: negative stride%s%s");
+  return EBR_OK;
+}
+
+// Rows of a chunk of the gradient: enough chunks to fill the GPU's warps about twice, 8 to 256 rows.
+int64_t grad_chunk_rows(int64_t n, int64_t C) {
+  const int64_t blocks = (C + 255) / 256;
+  int64_t r = 8;
+  while (r < 256 && n * blocks / r > 8192) r *= 2;
+  return r;
+}
+
+// ------------------------------------------------------------------------------------------------ distillation
+
+template <typename T, bool kStats>
+int launch_distill(const ebr::distill::Args& a, cudaStream_t st) {
+  using namespace ebr::distill;
+  constexpr int kFull = static_cast<int>(16 / sizeof(T));
+  int v = access_width(kFull, a.V, {{a.logits, a.logits_stride, int(sizeof(T))}, {a.grad, a.V, int(sizeof(T))}});
+  if (v != kFull) v = 1;
+  auto launch = [&](auto threads, auto vec) -> int {
+    constexpr int kThreads = decltype(threads)::value, kVec = decltype(vec)::value;
+    constexpr int kGroups = kThreads == 32 ? 8 : 1;
+    auto* kernel = distill_kernel<T, kThreads, kVec, kStats>;
+    const size_t smem = static_cast<size_t>(kGroups) * 2 * a.K * 4;
+    if (smem > 48 * 1024) {
+      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 static_cast<int>(smem));
+      if (e != cudaSuccess) return cuda_error(e, "distill attributes");
+    }
+    kernel<<<static_cast<unsigned>((a.N + kGroups - 1) / kGroups), kThreads * kGroups, smem, st>>>(a);
+    return check_launch("topk_distill");
+  };
+  using One = std::integral_constant<int, 1>;
+  using Full = std::integral_constant<int, kFull>;
+  using Warp = std::integral_constant<int, 32>;
+  using Block = std::integral_constant<int, 512>;
+  if (a.V <= 1024 && a.K <= 512) return v == kFull ? launch(Warp{}, Full{}) : launch(Warp{}, One{});
+  return v == kFull ? launch(Block{}, Full{}) : launch(Block{}, One{});
+}
+
+int check_distill(int dtype, int id_type, int top_dtype, int64_t N, int64_t V, int64_t K, double tau, int64_t stride) {
+  int rc = check_layer_dtype(dtype, false);
+  if (rc == EBR_OK) rc = check_layer_dtype(top_dtype, false);
+  if (rc == EBR_OK) rc = check_id_type(id_type);
+  if (rc != EBR_OK) return rc;
+  if (N < 0 || V < 1 || K < 1 || K > 4096) return set_error(EBR_ERR_SHAPE, "topk_distill: bad sizes%s%s");
+  if (N >= (int64_t{1} << 31) || V >= (int64_t{1} << 31)) return set_error(EBR_ERR_SHAPE, "topk_distill: size too large%s%s");
+  if (!(tau > 0.0) || tau > 1e30) return set_error(EBR_ERR_SHAPE, "topk_distill: the temperature must be positive%s%s");
+  if (stride < 0) return set_error(EBR_ERR_STRIDE, "topk_distill: negative stride%s%s");
+  return EBR_OK;
+}
+
+ebr::distill::Args distill_args(int64_t N, int64_t V, int64_t K, double tau, double factor, int id_type, int top_dtype,
+                                const void* logits, int64_t stride, const void* ids, const void* top,
+                                const float* row_weight) {
+  ebr::distill::Args a = {};
+  a.N = N;
+  a.V = V;
+  a.K = static_cast<int>(K);
+  a.tau = static_cast<float>(tau);
+  a.inv_tau = static_cast<float>(1.0 / tau);
+  a.exp2_scale = static_cast<float>(1.4426950408889634 / tau);
+  a.factor = static_cast<float>(factor);
+  a.logits = logits;
+  a.logits_stride = stride;
+  a.top_ids = ids;
+  a.ids64 = id_type == EBR_INT64;
+  a.top_logits = top;
+  a.top_dtype = top_dtype;
+  a.row_weight = row_weight;
+  return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+int ebr_scaled_embedding(int w_dtype, int out_dtype, int id_type, int64_t n, int64_t V, int64_t C, double scale,
+                         const void* ids, const void* w, int64_t w_stride, void* out, void* stream) {
+  int rc = check_embedding(id_type, n, V, C, w_stride);
+  if (rc == EBR_OK) rc = check_layer_dtype(w_dtype, false);
+  if (rc == EBR_OK) rc = check_layer_dtype(out_dtype, false);
+  if (rc != EBR_OK) return rc;
+  if (n == 0) return EBR_OK;
+  if (!ids || !w || !out) return set_error(EBR_ERR_NULL, "scaled_embedding: NULL pointer%s%s");
+  int device = 0;
+  if ((rc = check_device(&device)) != EBR_OK) return rc;
+  auto st = static_cast<cudaStream_t>(stream);
+  return with_types(w_dtype, out_dtype, [&](auto* wt, auto* ot) -> int {
+    using TW = std::remove_pointer_t<decltype(wt)>;
+    using TO = std::remove_pointer_t<decltype(ot)>;
+    const int most = sizeof(TW) == 4 && sizeof(TO) == 4 ? 4 : 8;
+    const int v = access_width(most, C, {{w, w_stride, int(sizeof(TW))}, {out, C, int(sizeof(TO))}});
+    return with_width(v, [&](auto vc) -> int {
+      constexpr int V_ = decltype(vc)::value;
+      using namespace ebr::embed;
+      const int64_t cols = (C + 32 * V_ - 1) / (32 * V_);
+      const int64_t want = (n + kLookupWarps - 1) / kLookupWarps;
+      const int64_t cap = std::max<int64_t>(1, (want + kLookupRows - 1) / kLookupRows);
+      const int64_t grid = want * cols <= static_cast<int64_t>(sm_count(device)) * 8 ? want : cap;
+      if (cols > 65535) return set_error(EBR_ERR_SHAPE, "scaled_embedding: row too long%s%s");
+      lookup_kernel<TW, TO, V_><<<dim3(static_cast<unsigned>(grid), static_cast<unsigned>(cols)), kLookupWarps * 32, 0,
+                                  st>>>(IdSource{ids, id_type == EBR_INT64, static_cast<int>(V)}, n, C,
+                                        static_cast<float>(scale), static_cast<const TW*>(w), w_stride,
+                                        static_cast<TO*>(out));
+      return check_launch("scaled_embedding");
+    });
+  });
+}
+
+size_t ebr_scaled_embedding_grad_scratch_bytes(int64_t n, int64_t V, int64_t C) {
+  if (n <= 0 || V < 1 || C < 1 || n >= kMaxSortKeys || V >= kMaxSortKeys || C > (1 << 24)) return 0;
+  const int passes = digit_passes(V);
+  const int64_t chunks = (n + grad_chunk_rows(n, C) - 1) / grad_chunk_rows(n, C);
+  return sort_scratch(n, int64_t{1} << digit_bits(V, passes), passes, false) +
+         round16(static_cast<size_t>(chunks) * 2 * C * 4);
+}
+
+int ebr_scaled_embedding_grad(int g_dtype, int w_dtype, int id_type, int64_t n, int64_t V, int64_t C, double scale,
+                              const void* ids, const void* g, int64_t g_stride, void* dw, void* scratch,
+                              size_t scratch_bytes, void* stream) {
+  int rc = check_embedding(id_type, n, V, C, g_stride);
+  if (rc == EBR_OK) rc = check_layer_dtype(g_dtype, false);
+  if (rc == EBR_OK) rc = check_layer_dtype(w_dtype, false);
+  if (rc != EBR_OK) return rc;
+  if (!dw) return set_error(EBR_ERR_NULL, "scaled_embedding_grad: NULL pointer%s%s");
+  const int64_t dw_bytes = V * C * static_cast<int64_t>(elem_size(w_dtype));
+  auto st = static_cast<cudaStream_t>(stream);
+  int device = 0;
+  if (n == 0) {
+    if ((rc = check_device(&device)) != EBR_OK) return rc;
+    const cudaError_t e = cudaMemsetAsync(dw, 0, static_cast<size_t>(dw_bytes), st);
+    return e == cudaSuccess ? EBR_OK : cuda_error(e, "scaled_embedding_grad");
+  }
+  if (!ids || !g) return set_error(EBR_ERR_NULL, "scaled_embedding_grad: NULL pointer%s%s");
+  if (!scratch || !aligned16(scratch) || scratch_bytes < ebr_scaled_embedding_grad_scratch_bytes(n, V, C))
+    return set_error(EBR_ERR_SCRATCH, "scaled_embedding_grad: scratch too small or unaligned%s%s");
+  if ((rc = check_device(&device)) != EBR_OK) return rc;
+  const int passes = digit_passes(V), bits = digit_bits(V, passes);
+  int *key = nullptr, *order = nullptr;
+  const IdSource src{ids, id_type == EBR_INT64, static_cast<int>(V)};
+  rc = run_sort(device, src, n, passes, bits, {}, scratch, &key, &order, dw, dw_bytes, st);
+  if (rc != EBR_OK) return rc;
+  float* part = reinterpret_cast<float*>(static_cast<char*>(scratch) +
+                                         sort_scratch(n, int64_t{1} << bits, passes, false));
+  const int R = static_cast<int>(grad_chunk_rows(n, C));
+  const int64_t chunks = (n + R - 1) / R;
+  return with_types(g_dtype, w_dtype, [&](auto* gt, auto* wt) -> int {
+    using TG = std::remove_pointer_t<decltype(gt)>;
+    using TW = std::remove_pointer_t<decltype(wt)>;
+    using namespace ebr::embed;
+    const int most = sizeof(TG) == 4 ? 4 : 8;
+    const int v = access_width(most, C, {{g, g_stride, int(sizeof(TG))}, {dw, C, int(sizeof(TW))}, {part, C, 4}});
+    int r = with_width(v, [&](auto vc) -> int {
+      constexpr int V_ = decltype(vc)::value;
+      const int64_t cols = (C + 32 * V_ - 1) / (32 * V_);
+      if (cols > 65535) return set_error(EBR_ERR_SHAPE, "scaled_embedding_grad: row too long%s%s");
+      grad_chunk_kernel<TG, TW, V_><<<dim3(static_cast<unsigned>((chunks + kGradWarps - 1) / kGradWarps),
+                                           static_cast<unsigned>(cols)), kGradWarps * 32, 0, st>>>(
+          static_cast<int>(n), static_cast<int>(V), C, R, key, order, static_cast<const TG*>(g), g_stride,
+          static_cast<float>(scale), static_cast<TW*>(dw), part);
+      return check_launch("scaled_embedding_grad");
+    });
+    if (r != EBR_OK || chunks == 1) return r;
+    const int64_t cols = (C + 127) / 128;
+    if (cols > 65535) return set_error(EBR_ERR_SHAPE, "scaled_embedding_grad: row too long%s%s");
+    grad_join_kernel<TW><<<dim3(static_cast<unsigned>((chunks + kJoinChunks - 1) / kJoinChunks),
+                                static_cast<unsigned>(cols)), kJoinWarps * 32, 0, st>>>(
+        static_cast<int>(n), static_cast<int>(V), C, R, static_cast<int>(chunks), key, static_cast<float>(scale),
+        static_cast<TW*>(dw), part);
+    return check_launch("scaled_embedding_grad join");
+  });
+}
+
+size_t ebr_expert_route_scratch_bytes(int64_t T, int64_t K, int64_t E) {
+  if (T <= 0 || K <= 0 || E < 1 || E > kMaxExperts || T >= kMaxSortKeys || K >= kMaxSortKeys || T * K >= kMaxSortKeys)
+    return 0;
+  return sort_scratch(T * K, E, 1, true);
+}
+
+int ebr_expert_route(int id_type, int64_t T, int64_t K, int64_t E, int64_t capacity, const void* ids, int32_t* row_of,
+                     int32_t* slot_of, int32_t* offsets, void* scratch, size_t scratch_bytes, void* stream) {
+  int rc = check_id_type(id_type);
+  if (rc != EBR_OK) return rc;
+  if (T < 0 || K < 1 || E < 1 || E > kMaxExperts || capacity < 0) return set_error(EBR_ERR_SHAPE, "expert_route: bad sizes%s%s");
+  if (T >= kMaxSortKeys || K >= kMaxSortKeys || T * K >= kMaxSortKeys || capacity >= kMaxSortKeys ||
+      E * capacity >= kMaxSortKeys)
+    return set_error(EBR_ERR_SHAPE, "expert_route: size too large%s%s");
+  const int64_t n = T * K, rows = capacity ? E * capacity : n;
+  if (!offsets || (n && (!ids || !row_of)) || (rows && !slot_of)) return set_error(EBR_ERR_NULL, "expert_route: NULL pointer%s%s");
+  const size_t need = ebr_expert_route_scratch_bytes(T, K, E);
+  if (need && (!scratch || !aligned16(scratch) || scratch_bytes < need))
+    return set_error(EBR_ERR_SCRATCH, "expert_route: scratch too small or unaligned%s%s");
+  int device = 0;
+  if ((rc = check_device(&device)) != EBR_OK) return rc;
+  int bits = 0;
+  while ((1 << bits) < E) ++bits;
+  ebr::keysort::RouteOut route = {};
+  route.row_of = row_of ? row_of : offsets;  // no slot: only marks the sort as a route
+  route.slot_of = slot_of;
+  route.offsets = offsets;
+  route.experts = static_cast<int>(E);
+  route.capacity = capacity;
+  route.rows = rows;
+  return run_sort(device, IdSource{ids, id_type == EBR_INT64, static_cast<int>(E)}, n, 1, bits, route, scratch, nullptr,
+                  nullptr, nullptr, 0, static_cast<cudaStream_t>(stream));
+}
+
+int ebr_expert_scatter(int dtype, int weight_dtype, int64_t T, int64_t K, int64_t C, int64_t rows, const void* x,
+                       int64_t x_stride, const int32_t* row_of, const int32_t* slot_of, const void* weights,
+                       const void* rows_in, void* rows_out, void* dots, void* stream) {
+  int rc = check_layer_dtype(dtype, false);
+  if (rc != EBR_OK) return rc;
+  if (weight_dtype != EBR_FLOAT32 && weight_dtype != dtype)
+    return set_error(EBR_ERR_DTYPE, "expert_scatter: weights must be float32 or of the rows' type%s%s");
+  if (T < 0 || K < 1 || C < 1 || rows < 0 || T >= kMaxSortKeys || K >= kMaxSortKeys || T * K >= kMaxSortKeys ||
+      rows >= kMaxSortKeys || C > (1 << 24))
+    return set_error(EBR_ERR_SHAPE, "expert_scatter: bad sizes%s%s");
+  if (x_stride < 0) return set_error(EBR_ERR_STRIDE, "expert_scatter: negative stride%s%s");
+  if (!rows_out && !dots) return set_error(EBR_ERR_NULL, "expert_scatter: no output%s%s");
+  if ((rows_in == nullptr) != (dots == nullptr) && T * rows != 0)
+    return set_error(EBR_ERR_NULL, "expert_scatter: rows_in and dots go together%s%s");
+  if ((T && (!x || !row_of)) || (rows && rows_out && !slot_of)) return set_error(EBR_ERR_NULL, "expert_scatter: NULL pointer%s%s");
+  if (T == 0 && (rows == 0 || !rows_out)) return EBR_OK;
+  int device = 0;
+  if ((rc = check_device(&device)) != EBR_OK) return rc;
+  auto st = static_cast<cudaStream_t>(stream);
+  return with_type(dtype, [&](auto* tag) -> int {
+    using T_ = std::remove_pointer_t<decltype(tag)>;
+    if constexpr (std::is_same_v<T_, double>) {
+      return EBR_ERR_DTYPE;
+    } else {
+      const int size = sizeof(T_);
+      const int v = access_width(16 / size, C, {{x, x_stride, size}, {rows_in, C, size}, {rows_out, C, size}});
+      return with_width(v, [&](auto vc) -> int {
+        constexpr int V_ = decltype(vc)::value;
+        auto launch = [&](auto* wtag, auto with_dots) -> int {
+          using TW = std::remove_pointer_t<decltype(wtag)>;
+          using namespace ebr::experts;
+          const int64_t tb = (T + kWarps - 1) / kWarps;
+          const int64_t zb = rows_out ? (rows + kZeroRows - 1) / kZeroRows : 0;
+          scatter_kernel<T_, TW, V_, decltype(with_dots)::value><<<static_cast<unsigned>(tb + zb), kWarps * 32, 0, st>>>(
+              T, static_cast<int>(K), C, rows, static_cast<const T_*>(x), x_stride, row_of, slot_of,
+              static_cast<const TW*>(weights), static_cast<const T_*>(rows_in), static_cast<T_*>(rows_out),
+              static_cast<TW*>(dots), static_cast<int>(tb));
+          return check_launch("expert_scatter");
+        };
+        if (weight_dtype == EBR_FLOAT32)
+          return dots ? launch(static_cast<float*>(nullptr), std::true_type{})
+                      : launch(static_cast<float*>(nullptr), std::false_type{});
+        return dots ? launch(static_cast<T_*>(nullptr), std::true_type{})
+                    : launch(static_cast<T_*>(nullptr), std::false_type{});
+      });
+    }
+  });
+}
+
+int ebr_expert_combine(int dtype, int weight_dtype, int64_t T, int64_t K, int64_t C, const void* rows_in,
+                       int64_t rows_stride, const int32_t* row_of, const void* weights, void* y, void* stream) {
+  int rc = check_layer_dtype(dtype, false);
+  if (rc != EBR_OK) return rc;
+  if (weight_dtype != EBR_FLOAT32 && weight_dtype != dtype)
+    return set_error(EBR_ERR_DTYPE, "expert_combine: weights must be float32 or of the rows' type%s%s");
+  if (T < 0 || K < 1 || C < 1 || T >= kMaxSortKeys || K >= kMaxSortKeys || T * K >= kMaxSortKeys || C > (1 << 24))
+    return set_error(EBR_ERR_SHAPE, "expert_combine: bad sizes%s%s");
+  if (rows_stride < 0) return set_error(EBR_ERR_STRIDE, "expert_combine: negative stride%s%s");
+  if (T == 0) return EBR_OK;
+  if (!row_of || !y) return set_error(EBR_ERR_NULL, "expert_combine: NULL pointer%s%s");
+  int device = 0;
+  if ((rc = check_device(&device)) != EBR_OK) return rc;
+  auto st = static_cast<cudaStream_t>(stream);
+  return with_type(dtype, [&](auto* tag) -> int {
+    using T_ = std::remove_pointer_t<decltype(tag)>;
+    if constexpr (std::is_same_v<T_, double>) {
+      return EBR_ERR_DTYPE;
+    } else {
+      const int size = sizeof(T_);
+      const int v = access_width(16 / size, C, {{rows_in, rows_stride, size}, {y, C, size}});
+      return with_width(v, [&](auto vc) -> int {
+        constexpr int V_ = decltype(vc)::value;
+        auto launch = [&](auto* wtag) -> int {
+          using TW = std::remove_pointer_t<decltype(wtag)>;
+          using namespace ebr::experts;
+          combine_kernel<T_, TW, V_><<<static_cast<unsigned>((T + kWarps - 1) / kWarps), kWarps * 32, 0, st>>>(
+              T, static_cast<int>(K), C, static_cast<const T_*>(rows_in), rows_stride, row_of,
+              static_cast<const TW*>(weights), static_cast<T_*>(y));
+          return check_launch("expert_combine");
+        };
+        return weight_dtype == EBR_FLOAT32 ? launch(static_cast<float*>(nullptr)) : launch(static_cast<T_*>(nullptr));
+      });
+    }
+  });
+}
+
+int ebr_topk_distill(int dtype, int id_type, int top_dtype, int64_t N, int64_t V, int64_t K, double tau, double factor,
+                     const void* logits, int64_t logits_stride, const void* top_ids, const void* top_logits,
+                     const float* row_weight, float* losses, float* stats, float* total, void* grad, void* stream) {
+  int rc = check_distill(dtype, id_type, top_dtype, N, V, K, tau, logits_stride);
+  if (rc != EBR_OK) return rc;
+  if (N == 0 && !total) return EBR_OK;
+  if (N && (!logits || !top_ids || !top_logits || !losses)) return set_error(EBR_ERR_NULL, "topk_distill: NULL pointer%s%s");
+  int device = 0;
+  if ((rc = check_device(&device)) != EBR_OK) return rc;
+  auto st = static_cast<cudaStream_t>(stream);
+  if (N) {
+    ebr::distill::Args a = distill_args(N, V, K, tau, factor, id_type, top_dtype, logits, logits_stride, top_ids,
+                                        top_logits, row_weight);
+    a.losses = losses;
+    a.stats = stats;
+    a.grad = grad;
+    rc = with_type(dtype, [&](auto* tag) -> int {
+      using T = std::remove_pointer_t<decltype(tag)>;
+      if constexpr (std::is_same_v<T, double>) return EBR_ERR_DTYPE;
+      else return launch_distill<T, true>(a, st);
+    });
+    if (rc != EBR_OK) return rc;
+  }
+  if (!total) return EBR_OK;
+  ebr::distill::total_kernel<<<1, 1024, 0, st>>>(N, static_cast<float>(factor), losses, total);
+  return check_launch("topk_distill total");
+}
+
+int ebr_topk_distill_grad(int dtype, int id_type, int top_dtype, int64_t N, int64_t V, int64_t K, double tau,
+                          double factor, const void* logits, int64_t logits_stride, const void* top_ids,
+                          const void* top_logits, const float* row_weight, const float* stats, const float* upstream,
+                          int64_t upstream_stride, int unless_one, void* grad, void* stream) {
+  int rc = check_distill(dtype, id_type, top_dtype, N, V, K, tau, logits_stride);
+  if (rc != EBR_OK) return rc;
+  if (upstream_stride != 0 && upstream_stride != 1) return set_error(EBR_ERR_STRIDE, "topk_distill_grad: upstream stride must be 0 or 1%s%s");
+  if (N == 0) return EBR_OK;
+  if (!logits || !top_ids || !top_logits || !stats || !upstream || !grad)
+    return set_error(EBR_ERR_NULL, "topk_distill_grad: NULL pointer%s%s");
+  int device = 0;
+  if ((rc = check_device(&device)) != EBR_OK) return rc;
+  ebr::distill::Args a = distill_args(N, V, K, tau, factor, id_type, top_dtype, logits, logits_stride, top_ids,
+                                      top_logits, row_weight);
+  a.stats = const_cast<float*>(stats);
+  a.upstream = upstream;
+  a.upstream_stride = upstream_stride;
+  a.unless_one = unless_one && upstream_stride == 0;
+  a.grad = grad;
+  return with_type(dtype, [&](auto* tag) -> int {
+    using T = std::remove_pointer_t<decltype(tag)>;
+    if constexpr (std::is_same_v<T, double>) return EBR_ERR_DTYPE;
+    else return launch_distill<T, false>(a, static_cast<cudaStream_t>(stream));
+  });
+}
+
+}  // extern "C"

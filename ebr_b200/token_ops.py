@@ -1,0 +1,453 @@
+"""Operators driven by integer ids next to the energy network (``include/ebr_tokens.h``): what a training step does with
+tokens before the first layer, inside a sparse layer and after the last one.
+
+* ``scaled_embedding(tokens, weight, scale)``: ``scale * weight[tokens]`` with one rounding, from the float32 master table
+  or a 16-bit one. Its gradient is a sum over the tokens sorted by id: no atomics, the same bits each time.
+* ``expert_route(expert_ids, experts)`` sorts a router's choices by expert; ``expert_dispatch(x, route)`` copies tokens to
+  their experts' rows and ``expert_combine(rows, route, weights)`` adds the rows back, weighted. Differentiable to every
+  order (the network's energy gradient is itself differentiated in training): the adjoints are the same kernels.
+* ``topk_distill_loss(logits, teacher_ids, teacher_logits)``: the Kullback-Leibler divergence from a teacher that is given
+  by its top logits, per row or reduced. A reduced loss makes its gradient in the forward pass, where the logits are at hand.
+
+All run the kernels of ``libebr_attn.so`` on the current CUDA stream, in float32 arithmetic with fixed summation orders.
+An id outside its range is a padding id everywhere: a zero row, no expert, no entry. CUDA only: a CPU tensor is an error.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Optional, Tuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from ebr_b200 import _native
+
+Tensor = torch.Tensor
+
+_DTYPES = {
+    torch.float32: _native.FLOAT32,
+    torch.float16: _native.FLOAT16,
+    torch.bfloat16: _native.BFLOAT16,
+}
+_IDS = {torch.int32: _native.INT32, torch.int64: _native.INT64}
+
+
+# ---------------------------------------------------------------------------------------------------- plumbing
+
+
+def _require(t: Tensor, what: str, name: str, types: dict, device: Optional[torch.device] = None) -> None:
+    if not t.is_cuda:
+        raise RuntimeError(f"{what} runs only on CUDA (sm_100a) tensors, got {name} on {t.device}; there is no CPU path")
+    if t.dtype not in types:
+        raise TypeError(f"{what}: unsupported dtype {t.dtype} of {name}")
+    if device is not None and t.device != device:
+        raise ValueError(f"{what}: {name} is on {t.device}, the other tensors are on {device}")
+
+
+def _call(what: str, device: torch.device, fn, *args) -> None:
+    """``fn(*args, stream)`` on ``device``'s current stream (the C ABI launches on the current device)."""
+    if device.index == torch.cuda.current_device():
+        status = fn(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            status = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if status:
+        _native.check(status, what)
+
+
+def _row_view(t: Tensor) -> Tuple[Tensor, int]:
+    """(tensor, row stride) of ``t`` [..., C] seen as rows of C unit-stride elements; copies where it is not such a view."""
+    c = t.shape[-1]
+    if t.is_contiguous():
+        return t, c
+    if t.dim() == 2 and (t.stride(1) == 1 or c == 1) and t.stride(0) >= 0:
+        return t, t.stride(0)
+    return t.contiguous(), c
+
+
+def _scratch(nbytes: int, device: torch.device) -> Optional[Tensor]:
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _ptr(t: Optional[Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+# ---------------------------------------------------------------------------------------------------- embedding
+
+
+def _lookup(tokens: Tensor, weight: Tensor, scale: float, dtype: torch.dtype) -> Tensor:
+    weight, stride = _row_view(weight)
+    v, c = weight.shape
+    out = torch.empty((*tokens.shape, c), device=weight.device, dtype=dtype)
+    _call("scaled_embedding", weight.device, _native.lib().ebr_scaled_embedding, _DTYPES[weight.dtype], _DTYPES[dtype],
+          _IDS[tokens.dtype], tokens.numel(), v, c, scale, tokens.data_ptr(), weight.data_ptr(), stride,
+          out.data_ptr())  # fmt: skip
+    return out
+
+
+def _lookup_grad(tokens: Tensor, g: Tensor, scale: float, rows: int, dtype: torch.dtype) -> Tensor:
+    g, stride = _row_view(g)
+    n, c = tokens.numel(), g.shape[-1]
+    dw = torch.empty((rows, c), device=g.device, dtype=dtype)
+    lib = _native.lib()
+    nbytes = lib.ebr_scaled_embedding_grad_scratch_bytes(n, rows, c)
+    scratch = _scratch(nbytes, g.device)
+    _call("scaled_embedding_grad", g.device, lib.ebr_scaled_embedding_grad, _DTYPES[g.dtype], _DTYPES[dtype],
+          _IDS[tokens.dtype], n, rows, c, scale, tokens.data_ptr(), g.data_ptr(), stride, dw.data_ptr(), _ptr(scratch),
+          nbytes)  # fmt: skip
+    return dw
+
+
+class _Embed(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight: Tensor, tokens: Tensor, scale: float, dtype: torch.dtype) -> Tensor:
+        ctx.save_for_backward(tokens)
+        ctx.scale, ctx.rows, ctx.dtype = scale, weight.shape[0], weight.dtype
+        return _lookup(tokens, weight, scale, dtype)
+
+    @staticmethod
+    def backward(ctx, g: Tensor):
+        (tokens,) = ctx.saved_tensors
+        if torch.is_grad_enabled():
+            return _EmbedGrad.apply(g, tokens, ctx.scale, ctx.rows, ctx.dtype), None, None, None
+        return _lookup_grad(tokens, g, ctx.scale, ctx.rows, ctx.dtype), None, None, None
+
+
+class _EmbedGrad(torch.autograd.Function):
+    """The table's gradient as a function of the output's; linear, so its own backward is the lookup."""
+
+    @staticmethod
+    def forward(ctx, g: Tensor, tokens: Tensor, scale: float, rows: int, dtype: torch.dtype) -> Tensor:
+        ctx.save_for_backward(tokens)
+        ctx.scale, ctx.dtype = scale, g.dtype
+        return _lookup_grad(tokens, g, scale, rows, dtype)
+
+    @staticmethod
+    def backward(ctx, gg: Tensor):
+        (tokens,) = ctx.saved_tensors
+        return _Embed.apply(gg, tokens, ctx.scale, ctx.dtype), None, None, None, None
+
+
+def scaled_embedding(tokens: Tensor, weight: Tensor, scale: float = 1.0, dtype: Optional[torch.dtype] = None) -> Tensor:
+    """``round(scale * weight[tokens])``, ``[*tokens.shape, C]`` of ``dtype`` (default: ``weight``'s).
+
+    ``tokens``: int32 or int64 of any shape; an id outside ``[0, V)`` gives a row of zeros and no gradient. ``weight``
+    ``[V, C]``: float32, float16 or bfloat16. Differentiable in ``weight`` to every order; the gradient has its type and is
+    summed in float32."""
+    _require(weight, "scaled_embedding", "weight", _DTYPES)
+    _require(tokens, "scaled_embedding", "tokens", _IDS, weight.device)
+    if weight.dim() != 2 or not weight.shape[0] or not weight.shape[1]:
+        raise ValueError(f"scaled_embedding: weight must be [V, C], got {tuple(weight.shape)}")
+    dtype = weight.dtype if dtype is None else dtype
+    if dtype not in _DTYPES:
+        raise TypeError(f"scaled_embedding: unsupported output dtype {dtype}")
+    tokens = tokens.contiguous()
+    if torch.is_grad_enabled() and weight.requires_grad:
+        return _Embed.apply(weight, tokens, float(scale), dtype)
+    return _lookup(tokens, weight, float(scale), dtype)
+
+
+# ---------------------------------------------------------------------------------------------------- experts
+
+
+@dataclass(frozen=True)
+class ExpertRoute:
+    """Where each token's slots go (``expert_route``). ``row_of`` [*tokens, K]: the slot's row, -1 for a dropped one.
+    ``slot_of`` [rows]: the row's slot (token * K + k), -1 for a row of no slot. ``offsets`` [experts + 1]: the first
+    sorted position of each expert, counting every slot, so ``offsets[1:] - offsets[:-1]`` are the experts' loads; without
+    a capacity, expert e's rows are ``offsets[e]`` to ``offsets[e + 1]``. All int32 on the device."""
+
+    row_of: Tensor
+    slot_of: Tensor
+    offsets: Tensor
+    experts: int
+    capacity: Optional[int]
+
+    @property
+    def rows(self) -> int:
+        return self.slot_of.shape[0]
+
+    @property
+    def top_k(self) -> int:
+        return self.row_of.shape[-1]
+
+
+def expert_route(expert_ids: Tensor, experts: int, capacity: Optional[int] = None) -> ExpertRoute:
+    """Sort the slots of ``expert_ids`` [..., K] (int32 or int64) by expert, keeping their order within an expert.
+
+    Without ``capacity`` the experts' rows follow one another (``[tokens * K, C]`` buffers, the tail zero where ids are
+    invalid). With it, each expert owns ``capacity`` rows (``[experts * capacity, C]``, a batch for ``torch.bmm``), its
+    later slots are dropped and its unused rows are zero; nothing on the host depends on the loads, so the layer can be
+    captured in a CUDA graph. At most 1024 experts; an id outside ``[0, experts)`` is a dropped slot."""
+    _require(expert_ids, "expert_route", "expert_ids", _IDS)
+    if expert_ids.dim() < 1 or not expert_ids.shape[-1]:
+        raise ValueError(f"expert_route: expert_ids must be [..., K], got {tuple(expert_ids.shape)}")
+    if not 1 <= experts <= 1024:
+        raise ValueError(f"expert_route: 1 to 1024 experts, got {experts}")
+    if capacity is not None and capacity < 1:
+        raise ValueError(f"expert_route: the capacity must be positive, got {capacity}")
+    ids, dev = expert_ids.contiguous(), expert_ids.device
+    k, slots = ids.shape[-1], ids.numel()
+    rows = slots if capacity is None else experts * capacity
+    row_of = torch.empty(ids.shape, dtype=torch.int32, device=dev)
+    slot_of = torch.empty(rows, dtype=torch.int32, device=dev)
+    offsets = torch.empty(experts + 1, dtype=torch.int32, device=dev)
+    lib = _native.lib()
+    nbytes = lib.ebr_expert_route_scratch_bytes(slots // k, k, experts)
+    scratch = _scratch(nbytes, dev)
+    _call("expert_route", dev, lib.ebr_expert_route, _IDS[ids.dtype], slots // k, k, experts, capacity or 0,
+          ids.data_ptr(), row_of.data_ptr(), slot_of.data_ptr(), offsets.data_ptr(), _ptr(scratch), nbytes)  # fmt: skip
+    return ExpertRoute(row_of, slot_of, offsets, experts, capacity)
+
+
+def _weight_args(weights: Optional[Tensor], x: Tensor):
+    if weights is None:
+        return None, _native.FLOAT32
+    if weights.dtype != torch.float32 and weights.dtype != x.dtype:
+        weights = weights.float()
+    return weights.contiguous(), _DTYPES[weights.dtype]
+
+
+def _scatter(x: Tensor, route: ExpertRoute, weights: Optional[Tensor], rows_in: Optional[Tensor], want_rows: bool,
+             dots_dtype: Optional[torch.dtype] = None) -> Tuple[Optional[Tensor], Optional[Tensor]]:  # fmt: skip
+    x, stride = _row_view(x)
+    c = x.shape[-1]
+    weights, code = _weight_args(weights, x)
+    if weights is None and dots_dtype is not None:
+        code = _DTYPES[dots_dtype]
+    out = torch.empty((route.rows, c), device=x.device, dtype=x.dtype) if want_rows else None
+    dots = None
+    if rows_in is not None:
+        rows_in = rows_in.to(x.dtype).contiguous()
+        dots = torch.empty(route.row_of.shape, device=x.device, dtype=torch.float32 if code == _native.FLOAT32 else x.dtype)
+    _call("expert_scatter", x.device, _native.lib().ebr_expert_scatter, _DTYPES[x.dtype], code,
+          route.row_of.numel() // route.top_k, route.top_k, c, route.rows, x.data_ptr(), stride, route.row_of.data_ptr(),
+          route.slot_of.data_ptr(), _ptr(weights), _ptr(rows_in), _ptr(out), _ptr(dots))  # fmt: skip
+    return out, dots
+
+
+def _combine(rows: Tensor, route: ExpertRoute, weights: Optional[Tensor]) -> Tensor:
+    rows, stride = _row_view(rows)
+    c = rows.shape[-1]
+    weights, code = _weight_args(weights, rows)
+    y = torch.empty((*route.row_of.shape[:-1], c), device=rows.device, dtype=rows.dtype)
+    _call("expert_combine", rows.device, _native.lib().ebr_expert_combine, _DTYPES[rows.dtype], code,
+          route.row_of.numel() // route.top_k, route.top_k, c, rows.data_ptr(), stride, route.row_of.data_ptr(),
+          _ptr(weights), y.data_ptr())  # fmt: skip
+    return y
+
+
+class _Dispatch(torch.autograd.Function):
+    """rows[row_of[t, k]] = weights[t, k] * x[t] (weights None: ones). Its adjoints are the combine and the row dots."""
+
+    @staticmethod
+    def forward(ctx, x: Tensor, weights: Optional[Tensor], route: ExpertRoute) -> Tensor:
+        ctx.route = route
+        ctx.weighted = weights is not None
+        ctx.save_for_backward(*((x, weights) if ctx.weighted else ()))
+        return _scatter(x, route, weights, None, True)[0]
+
+    @staticmethod
+    def backward(ctx, g: Tensor):
+        route = ctx.route
+        x, weights = ctx.saved_tensors if ctx.weighted else (None, None)
+        gx = _Combine.apply(g, weights, route) if ctx.needs_input_grad[0] else None
+        gw = _RowDots.apply(x, g, route, weights.dtype) if ctx.weighted and ctx.needs_input_grad[1] else None
+        return gx, gw, None
+
+
+class _Combine(torch.autograd.Function):
+    """y[t] = sum_k weights[t, k] * rows[row_of[t, k]] (weights None: ones)."""
+
+    @staticmethod
+    def forward(ctx, rows: Tensor, weights: Optional[Tensor], route: ExpertRoute) -> Tensor:
+        ctx.route = route
+        ctx.weighted = weights is not None
+        ctx.save_for_backward(*((rows, weights) if ctx.weighted else ()))
+        return _combine(rows, route, weights)
+
+    @staticmethod
+    def backward(ctx, g: Tensor):
+        route = ctx.route
+        rows, weights = ctx.saved_tensors if ctx.weighted else (None, None)
+        need_rows, need_weights = ctx.needs_input_grad[:2]
+        if need_rows and need_weights and ctx.weighted and not torch.is_grad_enabled():
+            grows, gw = _scatter(g.to(rows.dtype), route, weights, rows, True)  # both in one pass over g and the rows
+            return grows, gw.to(weights.dtype), None
+        grows = _Dispatch.apply(g, weights, route) if need_rows else None
+        gw = _RowDots.apply(g, rows, route, weights.dtype) if ctx.weighted and need_weights else None
+        return grows, gw, None
+
+
+class _RowDots(torch.autograd.Function):
+    """dots[t, k] = <x[t], rows[row_of[t, k]]>: the gradient of the weights, bilinear in x and the rows."""
+
+    @staticmethod
+    def forward(ctx, x: Tensor, rows: Tensor, route: ExpertRoute, dtype: torch.dtype) -> Tensor:
+        ctx.route = route
+        ctx.save_for_backward(x, rows)
+        code = dtype if dtype in (torch.float32, x.dtype) else torch.float32
+        return _scatter(x, route, None, rows, False, code)[1].to(dtype)
+
+    @staticmethod
+    def backward(ctx, g: Tensor):
+        x, rows = ctx.saved_tensors
+        gx = _Combine.apply(rows, g, ctx.route) if ctx.needs_input_grad[0] else None
+        grows = _Dispatch.apply(x, g, ctx.route) if ctx.needs_input_grad[1] else None
+        return gx, grows, None, None
+
+
+def expert_dispatch(x: Tensor, route: ExpertRoute) -> Tensor:
+    """Each token's vector in the rows of its experts: ``[rows, C]`` with ``rows[route.row_of[t, k]] = x[t]`` and zeros in
+    rows of no slot. ``x`` [*tokens, C] in float32, float16 or bfloat16; differentiable to every order."""
+    _require(x, "expert_dispatch", "x", _DTYPES, route.row_of.device)
+    if x.dim() < 1 or x.shape[:-1] != route.row_of.shape[:-1] or not x.shape[-1]:
+        raise ValueError(
+            f"expert_dispatch: x must be [*{tuple(route.row_of.shape[:-1])}, C] for this route, got {tuple(x.shape)}"
+        )
+    if torch.is_grad_enabled() and x.requires_grad:
+        return _Dispatch.apply(x, None, route)
+    return _scatter(x, route, None, None, True)[0]
+
+
+def expert_combine(rows: Tensor, route: ExpertRoute, weights: Optional[Tensor] = None) -> Tensor:
+    """The experts' rows added back to their tokens: ``y[t] = sum_k weights[t, k] * rows[route.row_of[t, k]]`` (``weights``
+    None: ones), ``[*tokens, C]``, dropped slots adding nothing. ``rows`` [rows, C] in float32, float16 or bfloat16;
+    ``weights`` [*tokens, K] (float32 or the rows' type are read as they are). The sum is float32 with one rounding.
+    Differentiable in both to every order."""
+    _require(rows, "expert_combine", "rows", _DTYPES, route.row_of.device)
+    if rows.dim() != 2 or rows.shape[0] != route.rows or not rows.shape[1]:
+        raise ValueError(f"expert_combine: rows must be [{route.rows}, C] for this route, got {tuple(rows.shape)}")
+    if weights is not None:
+        _require(weights, "expert_combine", "weights", _DTYPES, rows.device)
+        if weights.shape != route.row_of.shape:
+            raise ValueError(
+                f"expert_combine: weights must be {tuple(route.row_of.shape)} for this route, got {tuple(weights.shape)}"
+            )
+    if torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad)):
+        return _Combine.apply(rows, weights, route)
+    return _combine(rows, route, weights)
+
+
+# ---------------------------------------------------------------------------------------------------- distillation
+
+
+class _Distill:
+    """One call's arguments, laid out for the C ABI."""
+
+    def __init__(self, logits: Tensor, ids: Tensor, top: Tensor, tau: float, row_weight: Optional[Tensor],
+                 factor: float) -> None:  # fmt: skip
+        self.shape = logits.shape
+        self.logits, self.stride = _row_view(logits)
+        self.ids, self.top, self.row_weight = ids, top, row_weight
+        self.rows, self.vocab, self.k = ids.numel() // ids.shape[-1], logits.shape[-1], ids.shape[-1]
+        self.tau, self.factor = tau, factor
+
+    def _args(self):
+        return (_DTYPES[self.logits.dtype], _IDS[self.ids.dtype], _DTYPES[self.top.dtype], self.rows, self.vocab, self.k,
+                self.tau, self.factor, self.logits.data_ptr(), self.stride, self.ids.data_ptr(), self.top.data_ptr(),
+                _ptr(self.row_weight))  # fmt: skip
+
+    def forward(self, stats: Optional[Tensor], total: Optional[Tensor], grad: Optional[Tensor]) -> Tensor:
+        dev = self.logits.device
+        losses = torch.empty(self.ids.shape[:-1], device=dev, dtype=torch.float32)
+        _call("topk_distill_loss", dev, _native.lib().ebr_topk_distill, *self._args(), losses.data_ptr(), _ptr(stats),
+              _ptr(total), _ptr(grad))  # fmt: skip
+        return losses
+
+    def gradient(self, stats: Tensor, upstream: Tensor, grad: Tensor, unless_one: bool) -> None:
+        _call("topk_distill_loss", self.logits.device, _native.lib().ebr_topk_distill_grad, *self._args(),
+              stats.data_ptr(), upstream.data_ptr(), 0 if upstream.numel() == 1 and upstream.dim() == 0 else 1,
+              int(unless_one), grad.data_ptr())  # fmt: skip
+
+    def new_grad(self) -> Tensor:
+        return torch.empty(self.shape, device=self.logits.device, dtype=self.logits.dtype)
+
+
+class _TopkDistill(torch.autograd.Function):
+    """Rows' losses (``reduced`` false) or their sum times the factor. A reduced loss writes its gradient for an upstream of
+    1 in the forward pass, where a row's logits have just been read; the backward hands it out, and a kernel that reads
+    the real upstream on the device rewrites it from the logits only where that is not 1 (a loss scale, a mixed loss).
+    A further backward through the same graph gets a gradient of its own."""
+
+    @staticmethod
+    def forward(ctx, logits, ids, top, tau, row_weight, factor, reduced):
+        call = _Distill(logits, ids, top, tau, row_weight, factor)
+        dev = logits.device
+        stats = torch.empty((call.rows, 2), device=dev, dtype=torch.float32)
+        ctx.save_for_backward(logits, ids, top, row_weight, stats)
+        ctx.tau, ctx.factor, ctx.reduced, ctx.made = tau, factor, reduced, None
+        if not reduced:
+            return call.forward(stats, None, None)
+        total = torch.empty((), device=dev, dtype=torch.float32)
+        ctx.made = call.new_grad()
+        call.forward(stats, total, ctx.made)
+        return total
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g: Tensor):
+        logits, ids, top, row_weight, stats = ctx.saved_tensors
+        call = _Distill(logits, ids, top, ctx.tau, row_weight, ctx.factor)
+        grad, ctx.made = ctx.made, None
+        unless_one = grad is not None
+        if grad is None:
+            grad = call.new_grad()
+        call.gradient(stats, g.to(torch.float32).contiguous(), grad, unless_one)
+        return grad, None, None, None, None, None, None
+
+
+def topk_distill_loss(logits: Tensor, teacher_ids: Tensor, teacher_logits: Tensor, temperature: float = 1.0, *,
+                      row_weight: Optional[Tensor] = None, reduction: str = "mean") -> Tensor:  # fmt: skip
+    """Distillation from a teacher given by its top logits: for each row, ``temperature**2`` times the Kullback-Leibler
+    divergence of ``softmax(logits / temperature)`` from the softmax of the row's K teacher entries.
+
+    ``logits`` [..., V] in float32, float16 or bfloat16; ``teacher_ids`` [..., K] int32 or int64, an id outside ``[0, V)``
+    being no entry (a shorter list, a masked row); ``teacher_logits`` [..., K]; ``row_weight`` [...] multiplies the rows'
+    losses. A row without entries, or of weight 0, has loss 0 and gradient 0 whatever its logits hold. ``reduction``:
+    ``"none"`` (the rows' losses, float32), ``"sum"`` or ``"mean"`` (the sum over the number of rows). Differentiable once,
+    in ``logits``; the teacher and the weights are constants. A reduced loss keeps a gradient of the logits' size from the
+    forward to the backward pass."""
+    what = "topk_distill_loss"
+    _require(logits, what, "logits", _DTYPES)
+    _require(teacher_ids, what, "teacher_ids", _IDS, logits.device)
+    _require(teacher_logits, what, "teacher_logits", _DTYPES, logits.device)
+    if logits.dim() < 1 or teacher_ids.dim() < 1 or teacher_ids.shape[:-1] != logits.shape[:-1] or not logits.shape[-1]:
+        raise ValueError(f"{what}: logits [..., V] and teacher_ids [..., K] must have the same rows, got "
+                         f"{tuple(logits.shape)} and {tuple(teacher_ids.shape)}")  # fmt: skip
+    if teacher_logits.shape != teacher_ids.shape or not 1 <= teacher_ids.shape[-1] <= 4096:
+        raise ValueError(f"{what}: teacher_logits must be shaped as teacher_ids with 1 to 4096 entries a row, got "
+                         f"{tuple(teacher_logits.shape)} and {tuple(teacher_ids.shape)}")  # fmt: skip
+    if not temperature > 0:
+        raise ValueError(f"{what}: the temperature must be positive, got {temperature}")
+    if reduction not in ("none", "sum", "mean"):
+        raise ValueError(f"{what}: reduction must be 'none', 'sum' or 'mean', got {reduction!r}")
+    if teacher_logits.requires_grad or (row_weight is not None and row_weight.requires_grad):
+        raise ValueError(f"{what}: the teacher and the row weights are constants; detach them")
+    if row_weight is not None:
+        _require(row_weight, what, "row_weight", _DTYPES, logits.device)
+        if row_weight.shape != logits.shape[:-1]:
+            raise ValueError(f"{what}: row_weight must be {tuple(logits.shape[:-1])}, got {tuple(row_weight.shape)}")
+        row_weight = row_weight.to(torch.float32).contiguous()
+    ids, top = teacher_ids.contiguous(), teacher_logits.contiguous()
+    rows = ids.numel() // ids.shape[-1]
+    factor = 1.0 / rows if reduction == "mean" and rows else 1.0
+    reduced = reduction != "none"
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _TopkDistill.apply(logits, ids, top, float(temperature), row_weight, factor, reduced)
+    call = _Distill(logits, ids, top, float(temperature), row_weight, factor)
+    total = torch.empty((), device=logits.device, dtype=torch.float32) if reduced else None
+    losses = call.forward(None, total, None)
+    return total if reduced else losses
+
+
+__all__ = [
+    "ExpertRoute",
+    "expert_combine",
+    "expert_dispatch",
+    "expert_route",
+    "scaled_embedding",
+    "topk_distill_loss",
+]
