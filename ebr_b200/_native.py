@@ -143,9 +143,9 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.ebr_expert_route_scratch_bytes.argtypes = [i64, i64, i64]
     lib.ebr_expert_scatter.argtypes = [it, it, i64, i64, i64, i64, vp, i64, vp, vp, vp, vp, vp, vp, vp]
     lib.ebr_expert_combine.argtypes = [it, it, i64, i64, i64, vp, i64, vp, vp, vp, vp]
-    lib.ebr_topk_distill.argtypes = [it, it, it, i64, i64, i64, dbl, dbl, vp, i64, vp, vp, vp, vp, vp, vp, vp, vp]
+    lib.ebr_topk_distill.argtypes = [it, it, it, i64, i64, i64, dbl, dbl, vp, i64, vp, vp, vp, vp, vp, vp, vp, i64, vp]
     lib.ebr_topk_distill_grad.argtypes = [it, it, it, i64, i64, i64, dbl, dbl, vp, i64, vp, vp, vp, vp, vp, i64, it,
-                                          vp, vp]  # fmt: skip
+                                          vp, i64, vp]  # fmt: skip
     for name in EXPORTED_TOKENS:
         getattr(lib, name).restype = sz if name.endswith("_bytes") else ctypes.c_int
 

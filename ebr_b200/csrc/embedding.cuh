@@ -42,24 +42,27 @@ __device__ __forceinline__ void store_f(T* p, const float (&in)[V]) {
 
 // ------------------------------------------------------------------------------------------------ lookup
 
-// A warp writes one token's 32 vectors of columns (blockIdx.y picks them); kRows tokens' loads are in flight at once.
-constexpr int kLookupWarps = 8, kLookupRows = 4;
+// A warp writes up to 32 consecutive tokens' parts of 32 vectors of columns (blockIdx.y picks them): its lanes read the
+// ids at once, and kLookupAhead rows are in flight, so that the chain id -> row -> store is paid once for many rows.
+constexpr int kLookupWarps = 8, kLookupAhead = 4;
 
 template <typename TW, typename TO, int V>
 __global__ void __launch_bounds__(kLookupWarps * 32) lookup_kernel(IdSource src, int64_t n, int64_t C, float scale,
                                                                    const TW* __restrict__ w, int64_t w_stride,
-                                                                   TO* __restrict__ out) {
+                                                                   TO* __restrict__ out, int per_warp) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t c = (static_cast<int64_t>(blockIdx.y) * 32 + lane) * V;
-  if (c >= C) return;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kLookupWarps;
-  for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * kLookupWarps + warp; t0 < n; t0 += step * kLookupRows) {
-    float v[kLookupRows][V];
+  const bool live = c < C;
+  const int64_t t0 = (static_cast<int64_t>(blockIdx.x) * kLookupWarps + warp) * per_warp;
+  const int tokens = static_cast<int>(min(static_cast<int64_t>(per_warp), n - t0));  // may be <= 0
+  const int my_id = lane < tokens ? src.key(t0 + lane) : src.range;
+  TO* dst = out + t0 * C + c;
+  for (int j0 = 0; j0 < tokens; j0 += kLookupAhead) {
+    float v[kLookupAhead][V];
 #pragma unroll
-    for (int u = 0; u < kLookupRows; ++u) {
-      const int64_t t = t0 + u * step;
-      const int id = t < n ? src.key(t) : src.range;
-      if (id < src.range) {
+    for (int u = 0; u < kLookupAhead; ++u) {
+      const int id = __shfl_sync(0xffffffffu, my_id, (j0 + u) & 31);
+      if (id < src.range && live && j0 + u < tokens) {
         load_f<TW, V>(w + id * w_stride + c, v[u]);
       } else {
 #pragma unroll
@@ -67,12 +70,11 @@ __global__ void __launch_bounds__(kLookupWarps * 32) lookup_kernel(IdSource src,
       }
     }
 #pragma unroll
-    for (int u = 0; u < kLookupRows; ++u) {
-      const int64_t t = t0 + u * step;
-      if (t >= n) break;
+    for (int u = 0; u < kLookupAhead; ++u) {
+      if (j0 + u >= tokens || !live) continue;
 #pragma unroll
       for (int i = 0; i < V; ++i) v[u][i] *= scale;
-      store_f<TO, V>(out + t * C + c, v[u]);
+      store_f<TO, V>(dst + (j0 + u) * C, v[u]);
     }
   }
 }
@@ -91,6 +93,7 @@ __global__ void __launch_bounds__(kGradWarps * 32) grad_chunk_kernel(int n, int 
                                                                      float scale, TW* __restrict__ dw,
                                                                      float* __restrict__ part) {
   constexpr int kAhead = 8;  // rows in flight
+  using Raw = layers::Pack<TG, V>;
   const int lane = threadIdx.x & 31;
   const int64_t chunk = static_cast<int64_t>(blockIdx.x) * kGradWarps + (threadIdx.x >> 5);
   const int64_t begin = chunk * R;
@@ -104,100 +107,150 @@ __global__ void __launch_bounds__(kGradWarps * 32) grad_chunk_kernel(int n, int 
   float acc[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) acc[i] = 0.f;
-  auto flush = [&](bool goes_on) {
-    if (!live) return;
-    if (head || goes_on) {
-      store_f<float, V>(part + (chunk * 2 + (head ? 0 : 1)) * C + c, acc);
-    } else {
+  auto add = [&](const Raw& r) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) acc[i] *= scale;
-      store_f<TW, V>(dw + cur * C + c, acc);
+    for (int i = 0; i < V; ++i) acc[i] += Elem<TG>::load(&r.e[i]);
+  };
+  auto flush = [&](bool goes_on) {
+    if (live) {
+      if (head || goes_on) {
+        store_f<float, V>(part + (chunk * 2 + (head ? 0 : 1)) * C + c, acc);
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] *= scale;
+        store_f<TW, V>(dw + cur * C + c, acc);
+      }
     }
+#pragma unroll
+    for (int i = 0; i < V; ++i) acc[i] = 0.f;
+    head = false;
   };
   for (int64_t r0 = begin; r0 < end; r0 += 32) {
     const int rows = static_cast<int>(min(static_cast<int64_t>(32), end - r0));
     const int my_key = lane < rows ? key[r0 + lane] : range;
     const int my_row = lane < rows ? order[r0 + lane] : 0;
-    for (int j0 = 0; j0 < rows; j0 += kAhead) {
-      float v[kAhead][V];
-      int k[kAhead];
+    const int valid = __popc(__ballot_sync(0xffffffffu, my_key < range));  // the first ones: the keys are sorted
+    for (int j0 = 0; j0 < valid; j0 += kAhead) {
+      Raw v[kAhead];
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
-        const int j = j0 + u;
-        k[u] = __shfl_sync(0xffffffffu, my_key, j & 31);
-        const int64_t row = __shfl_sync(0xffffffffu, my_row, j & 31);
-        if (j < rows && k[u] < range && live) {
-          load_f<TG, V>(g + row * g_stride + c, v[u]);
-        } else {
+        const int64_t row = __shfl_sync(0xffffffffu, my_row, (j0 + u) & 31);
+        v[u] = {};
+        if (j0 + u < valid && live) v[u] = *reinterpret_cast<const Raw*>(g + row * g_stride + c);
+      }
+      const int last = __shfl_sync(0xffffffffu, my_key, min(j0 + kAhead, valid) - 1);
+      if (last == cur) {  // one run: the rows past `valid` add zeros
 #pragma unroll
-          for (int i = 0; i < V; ++i) v[u][i] = 0.f;
+        for (int u = 0; u < kAhead; ++u) add(v[u]);
+      } else {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const int k = __shfl_sync(0xffffffffu, my_key, (j0 + u) & 31);
+          if (j0 + u >= valid) continue;
+          if (k != cur) {
+            flush(false);
+            cur = k;
+          }
+          add(v[u]);
         }
       }
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        if (j0 + u >= rows) break;
-        if (k[u] != cur) {
-          flush(false);
-          if (k[u] >= range) return;
-          cur = k[u];
-          head = false;
-#pragma unroll
-          for (int i = 0; i < V; ++i) acc[i] = 0.f;
-        }
-#pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] += v[u][i];
-      }
+    }
+    if (valid < rows) {  // the rest of the chunk, and all behind it, has ids of no table row
+      flush(false);
+      return;
     }
   }
   flush(end < n && key[end] == cur);
 }
 
-// Runs that cross chunks: a block looks at kJoinChunks chunk ends; where the run at a chunk's end started in that chunk
-// and goes on, the block adds its partials in chunk order (its warps take every kJoinWarps-th partial) for 32 vectors of
-// four columns.
-constexpr int kJoinWarps = 8, kJoinChunks = 32;
+// Runs that cross chunks. A block looks at the ends of kJoinChunks chunks, a warp at one of them: where the run at a
+// chunk's end started in that chunk and goes on, its partials are added in chunk order. A run of a few chunks is added by
+// its warp, 32 vectors of four columns; a long one by the whole block, every warp taking every kJoinWarps-th partial.
+constexpr int kJoinWarps = 32, kJoinChunks = 32, kJoinShort = 16;
 
 template <typename TW>
 __global__ void __launch_bounds__(kJoinWarps * 32) grad_join_kernel(int n, int range, int64_t C, int R, int chunks,
                                                                     const int* __restrict__ key, float scale,
                                                                     TW* __restrict__ dw,
                                                                     const float* __restrict__ part) {
+  constexpr int kAhead = 8;
   __shared__ float4 sums[kJoinWarps][32];
+  __shared__ int ids[kJoinChunks];
+  __shared__ int lasts[kJoinChunks];  // the last chunk of a long run, or -1
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * kJoinChunks;
-  bool owner = false;
-  int id = 0;
-  if (first + lane < chunks) {
-    const int64_t begin = (first + lane) * R, end = begin + R;
-    if (end < n) {
+  const int64_t c = (static_cast<int64_t>(blockIdx.y) * 32 + lane) * 4;
+  const bool whole = C % 4 == 0;
+  // the partials of chunks from, from + step, ... up to `last` of the run that starts in `owner`
+  auto gather = [&](int64_t owner, int64_t from, int64_t last, int step) {
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (c < C)
+      for (int64_t j0 = from; j0 <= last; j0 += kAhead * step) {
+        float4 v[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const int64_t j = j0 + u * step;
+          v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (j > last) continue;
+          const float* p = part + (j * 2 + (j == owner ? 1 : 0)) * C + c;
+          if (whole) {
+            v[u] = *reinterpret_cast<const float4*>(p);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (c + i < C) (&v[u].x)[i] = p[i];
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          s.x += v[u].x;
+          s.y += v[u].y;
+          s.z += v[u].z;
+          s.w += v[u].w;
+        }
+      }
+    return s;
+  };
+  auto put = [&](int id, const float4& s) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (c + i < C) dw[id * C + c + i] = Elem<TW>::to((&s.x)[i] * scale);
+  };
+  {
+    const int64_t chunk = first + warp, begin = chunk * R, end = begin + R;
+    int id = -1;
+    int64_t last = -1;
+    if (chunk < chunks && end < n) {
       id = key[end - 1];
-      owner = id < range && key[end] == id && (begin == 0 || key[begin - 1] != id);
+      if (id >= range || key[end] != id || (begin > 0 && key[begin - 1] == id)) id = -1;
+    }
+    if (id >= 0) {  // the last chunk that starts with this id: the keys at the chunks' starts are in order
+      int64_t lo = chunk + 1, hi = chunks - 1;
+      if (lo + kJoinShort <= hi && key[(lo + kJoinShort) * R] != id) hi = lo + kJoinShort;
+      while (lo < hi) {
+        const int64_t mid = (lo + hi + 1) / 2;
+        if (key[mid * R] == id) lo = mid; else hi = mid - 1;
+      }
+      last = lo;
+      if (last - chunk < kJoinShort) {
+        put(id, gather(chunk, chunk, last, 1));
+        last = -1;
+      }
+    }
+    if (lane == 0) {
+      ids[warp] = id;
+      lasts[warp] = static_cast<int>(last);
     }
   }
-  unsigned owners = __ballot_sync(0xffffffffu, owner);
-  const int64_t c = (static_cast<int64_t>(blockIdx.y) * 32 + lane) * 4;
-  while (owners) {
-    const int o = __ffs(owners) - 1;
-    owners &= owners - 1;
+  __syncthreads();
+  for (int o = 0; o < kJoinChunks; ++o) {
+    if (lasts[o] < 0) continue;
     const int64_t chunk = first + o;
-    const int k = __shfl_sync(0xffffffffu, id, o);
-    // the last chunk that starts with this id: the keys at the chunks' starts are in order
-    int64_t lo = chunk + 1, hi = chunks - 1;
-    while (lo < hi) {
-      const int64_t mid = (lo + hi + 1) / 2;
-      if (key[mid * R] == k) lo = mid; else hi = mid - 1;
-    }
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int64_t j = chunk + warp; j <= lo; j += kJoinWarps) {
-      const float* p = part + (j * 2 + (j == chunk ? 1 : 0)) * C;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (c + i < C) (&s.x)[i] += p[c + i];
-    }
+    float4 s = gather(chunk, chunk + warp, lasts[o], kJoinWarps);
     sums[warp][lane] = s;
     __syncthreads();
     if (warp == 0) {
-#pragma unroll
+#pragma unroll 8
       for (int w = 1; w < kJoinWarps; ++w) {
         const float4 t = sums[w][lane];
         s.x += t.x;
@@ -205,9 +258,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) grad_join_kernel(int n, int r
         s.z += t.z;
         s.w += t.w;
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (c + i < C) dw[k * C + c + i] = Elem<TW>::to((&s.x)[i] * scale);
+      put(ids[o], s);
     }
     __syncthreads();
   }

@@ -170,9 +170,8 @@ int run_sort(int device, IdSource src, int64_t n, int passes, int bits, const eb
     int ctas = 1;
     while (ctas < 16 && static_cast<int64_t>(ctas) * ebr::keysort::kSortThreads < n) ctas *= 2;
     const int64_t per_thread = ((n + ctas - 1) / ctas + ebr::keysort::kSortThreads - 1) / ebr::keysort::kSortThreads;
-    // zeroing CTAs: one for 64 KB, whole clusters, at most what fills the other SMs once
-    int64_t fill_ctas = fill ? std::min<int64_t>((fill_bytes + 65535) / 65536, sm_count(device)) : 0;
-    if (fill && fill_ctas == 0) fill_ctas = 1;
+    // zeroing CTAs: one for 128 KB, whole clusters; many, so that the SMs that the sort leaves free even out
+    const int64_t fill_ctas = fill ? std::min<int64_t>((fill_bytes + 131071) / 131072, 1 << 20) : 0;
     const int fill_clusters = static_cast<int>((fill_ctas + ctas - 1) / ctas);
     if (per_thread <= 1) return launch_cluster_sort<1>(device, a, ctas, bits, fill_clusters, st);
     if (per_thread <= 2) return launch_cluster_sort<2>(device, a, ctas, bits, fill_clusters, st);
@@ -223,52 +222,136 @@ int check_embedding(int id_type, int64_t n, int64_t V, int64_t C, int64_t stride
   return EBR_OK;
 }
 
-// Rows of a chunk of the gradient: enough chunks to fill the GPU's warps about twice, 8 to 256 rows.
+// Rows of a chunk of the gradient, 8 to 256: some 4,000 warps' worth of chunks.
 int64_t grad_chunk_rows(int64_t n, int64_t C) {
   const int64_t blocks = (C + 255) / 256;
   int64_t r = 8;
-  while (r < 256 && n * blocks / r > 8192) r *= 2;
+  while (r < 256 && n * blocks / r > 6000) r *= 2;
   return r;
 }
 
 // ------------------------------------------------------------------------------------------------ distillation
 
+constexpr int64_t kMaxVocabulary = int64_t{1} << 19;
+constexpr int kMaxEntries = 1024;
+
+// Rows of a few logits take four lanes each, rows of up to kWarpRowBytes a warp, longer ones a ring of chunks: bfloat16 at
+// 2.1 GB of logits and gradient, a warp takes 0.53 ms at V = 8,192 (the ring 0.72) and 0.57 at 16,384 (0.60).
+constexpr int64_t kWarpRowBytes = 16 * 1024;
+
+bool distill_few(int64_t V, int64_t K) { return V <= 32 && K <= 32; }
+
 template <typename T, bool kStats>
-int launch_distill(const ebr::distill::Args& a, cudaStream_t st) {
+int launch_distill_few(const ebr::distill::Args& a, cudaStream_t st) {
   using namespace ebr::distill;
-  constexpr int kFull = static_cast<int>(16 / sizeof(T));
-  int v = access_width(kFull, a.V, {{a.logits, a.logits_stride, int(sizeof(T))}, {a.grad, a.V, int(sizeof(T))}});
-  if (v != kFull) v = 1;
-  auto launch = [&](auto threads, auto vec) -> int {
-    constexpr int kThreads = decltype(threads)::value, kVec = decltype(vec)::value;
-    constexpr int kGroups = kThreads == 32 ? 8 : 1;
-    auto* kernel = distill_kernel<T, kThreads, kVec, kStats>;
-    const size_t smem = static_cast<size_t>(kGroups) * 2 * a.K * 4;
-    if (smem > 48 * 1024) {
-      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 static_cast<int>(smem));
-      if (e != cudaSuccess) return cuda_error(e, "distill attributes");
-    }
-    kernel<<<static_cast<unsigned>((a.N + kGroups - 1) / kGroups), kThreads * kGroups, smem, st>>>(a);
-    return check_launch("topk_distill");
-  };
-  using One = std::integral_constant<int, 1>;
-  using Full = std::integral_constant<int, kFull>;
-  using Warp = std::integral_constant<int, 32>;
-  using Block = std::integral_constant<int, 512>;
-  if (a.V <= 1024 && a.K <= 512) return v == kFull ? launch(Warp{}, Full{}) : launch(Warp{}, One{});
-  return v == kFull ? launch(Block{}, Full{}) : launch(Block{}, One{});
+  constexpr int kLanes = 4, kGroups = kSmallThreads / kLanes;
+  distill_small_kernel<T, kLanes, kStats><<<static_cast<unsigned>((a.N + kGroups - 1) / kGroups), kSmallThreads,
+                                            static_cast<size_t>(kGroups) * 2 * a.K * 4, st>>>(a);
+  return check_launch("topk_distill");
 }
 
-int check_distill(int dtype, int id_type, int top_dtype, int64_t N, int64_t V, int64_t K, double tau, int64_t stride) {
+template <typename T>
+bool distill_by_warp(int64_t V) {
+  return V * static_cast<int64_t>(sizeof(T)) <= kWarpRowBytes;
+}
+
+template <typename T, bool kStats>
+int launch_distill_warp(const ebr::distill::Args& a, cudaStream_t st) {
+  using namespace ebr::distill;
+  distill_warp_kernel<T, kStats><<<static_cast<unsigned>((a.N + kMidWarps - 1) / kMidWarps), kMidWarps * 32,
+                                   static_cast<size_t>(kMidWarps) * 12 * a.K, st>>>(a);
+  return check_launch("topk_distill");
+}
+
+template <typename T, int kWarps, int kU>
+int launch_distill_row(int device, const ebr::distill::Args& a, int slices, int granules, int slots, int per_sm,
+                       cudaStream_t st) {
+  auto* kernel = ebr::distill::distill_row_kernel<T, kWarps, kU>;
+  static std::atomic<bool> ready[kMaxDevices];
+  if (device >= kMaxDevices || !ready[device].load()) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 216 * 1024);
+    if (e != cudaSuccess) return cuda_error(e, "topk_distill attributes");
+    if (device < kMaxDevices) ready[device].store(true);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kWarps * 32 + 32);
+  cfg.dynamicSmemBytes = static_cast<size_t>(slots) * kWarps * kU * 512;
+  const int64_t clusters = std::max<int64_t>(1, std::min<int64_t>(a.N, per_sm * sm_count(device) / slices));
+  cfg.gridDim = dim3(static_cast<unsigned>(clusters * slices));
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim = {static_cast<unsigned>(slices), 1, 1};
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, static_cast<const float*>(a.losses), slices, granules, slots);
+  if (e != cudaSuccess) return cuda_error(e, "topk_distill");
+  return check_launch("topk_distill");
+}
+
+template <typename T, bool kLoss>
+int launch_distill_entries(const ebr::distill::Args& a, cudaStream_t st) {
+  using namespace ebr::distill;
+  distill_entries_kernel<T, kLoss><<<static_cast<unsigned>((a.N + kEntryWarps - 1) / kEntryWarps), kEntryWarps * 32,
+                                     static_cast<size_t>(kEntryWarps) * 3 * a.K * 4, st>>>(a);
+  return check_launch("topk_distill entries");
+}
+
+// 16-byte granules that a row of V elements may touch, whatever its first byte.
+template <typename T>
+int64_t row_granules(int64_t V) {
+  constexpr int64_t kE = 16 / sizeof(T);
+  return (V + 2 * (kE - 1)) / kE;
+}
+
+template <typename T>
+int launch_distill(int device, const ebr::distill::Args& a, cudaStream_t st) {
+  if (distill_few(a.V, a.K)) return launch_distill_few<T, true>(a, st);
+  if (distill_by_warp<T>(a.V)) return launch_distill_warp<T, true>(a, st);
+  const int64_t total = row_granules<T>(a.V);
+  int slices = 1;
+  while (slices < ebr::distill::kMaxSlices && a.N * slices < 2 * sm_count(device) && (total + slices - 1) / slices > 256)
+    slices *= 2;
+  const int granules = static_cast<int>((total + slices - 1) / slices);
+  // the rows' weights travel in `losses`, which the last kernel writes
+  ebr::distill::distill_weights_kernel<<<static_cast<unsigned>((a.N + 7) / 8), 256, 0, st>>>(a, a.losses);
+  int rc = check_launch("topk_distill weights");
+  if (rc != EBR_OK) return rc;
+  // Rows above 128 KB: rings of six 16 KB chunks, two on an SM, keep more of the row between the passes; shorter rows want
+  // more rows in flight: rings of four 8 KB chunks, six on an SM. bfloat16 at 2.1 GB: V = 131,072 takes 0.45 ms with the
+  // first, 0.53 with the second; V = 32,768 takes 0.56 and 0.50.
+  rc = granules > 8192 ? launch_distill_row<T, 8, 4>(device, a, slices, granules, 6, 2, st)
+                       : launch_distill_row<T, 4, 4>(device, a, slices, granules, 4, 6, st);
+  return rc != EBR_OK ? rc : launch_distill_entries<T, true>(a, st);
+}
+
+template <typename T>
+int launch_distill_grad(int device, const ebr::distill::Args& a, cudaStream_t st) {
+  if (distill_few(a.V, a.K)) return launch_distill_few<T, false>(a, st);
+  if (distill_by_warp<T>(a.V)) return launch_distill_warp<T, false>(a, st);
+  constexpr int kThreads = 256;
+  const int64_t total = row_granules<T>(a.V);
+  const int slices = static_cast<int>((total + 4095) / 4096);
+  const int64_t items = a.N * slices;
+  const int64_t most = static_cast<int64_t>(sm_count(device)) * (a.unless_one ? 8 : 64);
+  ebr::distill::distill_grad_kernel<T, kThreads>
+      <<<static_cast<unsigned>(std::min(items, most)), kThreads, 0, st>>>(
+          a, slices, static_cast<int>((total + slices - 1) / slices));
+  const int rc = check_launch("topk_distill_grad");
+  return rc != EBR_OK ? rc : launch_distill_entries<T, false>(a, st);
+}
+
+int check_distill(int dtype, int id_type, int top_dtype, int64_t N, int64_t V, int64_t K, double tau, int64_t stride,
+                  int64_t grad_stride) {
   int rc = check_layer_dtype(dtype, false);
   if (rc == EBR_OK) rc = check_layer_dtype(top_dtype, false);
   if (rc == EBR_OK) rc = check_id_type(id_type);
   if (rc != EBR_OK) return rc;
-  if (N < 0 || V < 1 || K < 1 || K > 4096) return set_error(EBR_ERR_SHAPE, "topk_distill: bad sizes%s%s");
-  if (N >= (int64_t{1} << 31) || V >= (int64_t{1} << 31)) return set_error(EBR_ERR_SHAPE, "topk_distill: size too large%s%s");
+  if (N < 0 || V < 1 || K < 1 || K > kMaxEntries) return set_error(EBR_ERR_SHAPE, "topk_distill: bad sizes%s%s");
+  if (N >= (int64_t{1} << 31) || V > kMaxVocabulary) return set_error(EBR_ERR_SHAPE, "topk_distill: size too large%s%s");
   if (!(tau > 0.0) || tau > 1e30) return set_error(EBR_ERR_SHAPE, "topk_distill: the temperature must be positive%s%s");
-  if (stride < 0) return set_error(EBR_ERR_STRIDE, "topk_distill: negative stride%s%s");
+  if (stride < 0 || grad_stride < V) return set_error(EBR_ERR_STRIDE, "topk_distill: bad row stride%s%s");
   return EBR_OK;
 }
 
@@ -317,14 +400,15 @@ int ebr_scaled_embedding(int w_dtype, int out_dtype, int id_type, int64_t n, int
       constexpr int V_ = decltype(vc)::value;
       using namespace ebr::embed;
       const int64_t cols = (C + 32 * V_ - 1) / (32 * V_);
-      const int64_t want = (n + kLookupWarps - 1) / kLookupWarps;
-      const int64_t cap = std::max<int64_t>(1, (want + kLookupRows - 1) / kLookupRows);
-      const int64_t grid = want * cols <= static_cast<int64_t>(sm_count(device)) * 8 ? want : cap;
       if (cols > 65535) return set_error(EBR_ERR_SHAPE, "scaled_embedding: row too long%s%s");
-      lookup_kernel<TW, TO, V_><<<dim3(static_cast<unsigned>(grid), static_cast<unsigned>(cols)), kLookupWarps * 32, 0,
-                                  st>>>(IdSource{ids, id_type == EBR_INT64, static_cast<int>(V)}, n, C,
-                                        static_cast<float>(scale), static_cast<const TW*>(w), w_stride,
-                                        static_cast<TO*>(out));
+      // as many tokens to a warp (up to 32) as leave some 24 warps for each SM
+      int per_warp = 1;
+      while (per_warp < 32 && n * cols / per_warp > 24 * static_cast<int64_t>(sm_count(device))) per_warp *= 2;
+      const int64_t blocks = (n + per_warp * kLookupWarps - 1) / (per_warp * kLookupWarps);
+      lookup_kernel<TW, TO, V_><<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(cols)), kLookupWarps * 32,
+                                  0, st>>>(IdSource{ids, id_type == EBR_INT64, static_cast<int>(V)}, n, C,
+                                           static_cast<float>(scale), static_cast<const TW*>(w), w_stride,
+                                           static_cast<TO*>(out), per_warp);
       return check_launch("scaled_embedding");
     });
   });
@@ -516,11 +600,12 @@ int ebr_expert_combine(int dtype, int weight_dtype, int64_t T, int64_t K, int64_
 
 int ebr_topk_distill(int dtype, int id_type, int top_dtype, int64_t N, int64_t V, int64_t K, double tau, double factor,
                      const void* logits, int64_t logits_stride, const void* top_ids, const void* top_logits,
-                     const float* row_weight, float* losses, float* stats, float* total, void* grad, void* stream) {
-  int rc = check_distill(dtype, id_type, top_dtype, N, V, K, tau, logits_stride);
+                     const float* row_weight, float* losses, float* stats, float* total, void* grad, int64_t grad_stride,
+                     void* stream) {
+  int rc = check_distill(dtype, id_type, top_dtype, N, V, K, tau, logits_stride, grad ? grad_stride : V);
   if (rc != EBR_OK) return rc;
   if (N == 0 && !total) return EBR_OK;
-  if (N && (!logits || !top_ids || !top_logits || !losses)) return set_error(EBR_ERR_NULL, "topk_distill: NULL pointer%s%s");
+  if (N && (!logits || !top_ids || !top_logits || !losses || !stats)) return set_error(EBR_ERR_NULL, "topk_distill: NULL pointer%s%s");
   int device = 0;
   if ((rc = check_device(&device)) != EBR_OK) return rc;
   auto st = static_cast<cudaStream_t>(stream);
@@ -530,10 +615,11 @@ int ebr_topk_distill(int dtype, int id_type, int top_dtype, int64_t N, int64_t V
     a.losses = losses;
     a.stats = stats;
     a.grad = grad;
+    a.grad_stride = grad_stride;
     rc = with_type(dtype, [&](auto* tag) -> int {
       using T = std::remove_pointer_t<decltype(tag)>;
       if constexpr (std::is_same_v<T, double>) return EBR_ERR_DTYPE;
-      else return launch_distill<T, true>(a, st);
+      else return launch_distill<T>(device, a, st);
     });
     if (rc != EBR_OK) return rc;
   }
@@ -545,8 +631,8 @@ int ebr_topk_distill(int dtype, int id_type, int top_dtype, int64_t N, int64_t V
 int ebr_topk_distill_grad(int dtype, int id_type, int top_dtype, int64_t N, int64_t V, int64_t K, double tau,
                           double factor, const void* logits, int64_t logits_stride, const void* top_ids,
                           const void* top_logits, const float* row_weight, const float* stats, const float* upstream,
-                          int64_t upstream_stride, int unless_one, void* grad, void* stream) {
-  int rc = check_distill(dtype, id_type, top_dtype, N, V, K, tau, logits_stride);
+                          int64_t upstream_stride, int unless_one, void* grad, int64_t grad_stride, void* stream) {
+  int rc = check_distill(dtype, id_type, top_dtype, N, V, K, tau, logits_stride, grad_stride);
   if (rc != EBR_OK) return rc;
   if (upstream_stride != 0 && upstream_stride != 1) return set_error(EBR_ERR_STRIDE, "topk_distill_grad: upstream stride must be 0 or 1%s%s");
   if (N == 0) return EBR_OK;
@@ -561,10 +647,11 @@ int ebr_topk_distill_grad(int dtype, int id_type, int top_dtype, int64_t N, int6
   a.upstream_stride = upstream_stride;
   a.unless_one = unless_one && upstream_stride == 0;
   a.grad = grad;
+  a.grad_stride = grad_stride;
   return with_type(dtype, [&](auto* tag) -> int {
     using T = std::remove_pointer_t<decltype(tag)>;
     if constexpr (std::is_same_v<T, double>) return EBR_ERR_DTYPE;
-    else return launch_distill<T, false>(a, static_cast<cudaStream_t>(stream));
+    else return launch_distill_grad<T>(device, a, static_cast<cudaStream_t>(stream));
   });
 }
 

@@ -350,20 +350,28 @@ class _Distill:
                 self.tau, self.factor, self.logits.data_ptr(), self.stride, self.ids.data_ptr(), self.top.data_ptr(),
                 _ptr(self.row_weight))  # fmt: skip
 
-    def forward(self, stats: Optional[Tensor], total: Optional[Tensor], grad: Optional[Tensor]) -> Tensor:
+    def forward(self, stats: Tensor, total: Optional[Tensor], grad: Optional[Tensor]) -> Tensor:
         dev = self.logits.device
         losses = torch.empty(self.ids.shape[:-1], device=dev, dtype=torch.float32)
-        _call("topk_distill_loss", dev, _native.lib().ebr_topk_distill, *self._args(), losses.data_ptr(), _ptr(stats),
-              _ptr(total), _ptr(grad))  # fmt: skip
+        _call("topk_distill_loss", dev, _native.lib().ebr_topk_distill, *self._args(), losses.data_ptr(), stats.data_ptr(),
+              _ptr(total), _ptr(grad), self._grad_stride(grad))  # fmt: skip
         return losses
 
     def gradient(self, stats: Tensor, upstream: Tensor, grad: Tensor, unless_one: bool) -> None:
         _call("topk_distill_loss", self.logits.device, _native.lib().ebr_topk_distill_grad, *self._args(),
               stats.data_ptr(), upstream.data_ptr(), 0 if upstream.numel() == 1 and upstream.dim() == 0 else 1,
-              int(unless_one), grad.data_ptr())  # fmt: skip
+              int(unless_one), grad.data_ptr(), self._grad_stride(grad))  # fmt: skip
 
     def new_grad(self) -> Tensor:
-        return torch.empty(self.shape, device=self.logits.device, dtype=self.logits.dtype)
+        """The gradient's buffer: contiguous, or with the logits' row stride where they are a view of slightly longer
+        rows (a padded vocabulary), so that both rows start at the same place of a 16-byte word."""
+        s = self.logits
+        if self.vocab < self.stride <= self.vocab + 256 and s.dim() == 2:
+            return torch.empty_strided(s.shape, s.stride(), device=s.device, dtype=s.dtype)
+        return torch.empty(self.shape, device=s.device, dtype=s.dtype)
+
+    def _grad_stride(self, grad: Optional[Tensor]) -> int:
+        return self.vocab if grad is None or grad.is_contiguous() else grad.stride(0)
 
 
 class _TopkDistill(torch.autograd.Function):
@@ -417,9 +425,11 @@ def topk_distill_loss(logits: Tensor, teacher_ids: Tensor, teacher_logits: Tenso
     if logits.dim() < 1 or teacher_ids.dim() < 1 or teacher_ids.shape[:-1] != logits.shape[:-1] or not logits.shape[-1]:
         raise ValueError(f"{what}: logits [..., V] and teacher_ids [..., K] must have the same rows, got "
                          f"{tuple(logits.shape)} and {tuple(teacher_ids.shape)}")  # fmt: skip
-    if teacher_logits.shape != teacher_ids.shape or not 1 <= teacher_ids.shape[-1] <= 4096:
-        raise ValueError(f"{what}: teacher_logits must be shaped as teacher_ids with 1 to 4096 entries a row, got "
+    if teacher_logits.shape != teacher_ids.shape or not 1 <= teacher_ids.shape[-1] <= 1024:
+        raise ValueError(f"{what}: teacher_logits must be shaped as teacher_ids with 1 to 1024 entries a row, got "
                          f"{tuple(teacher_logits.shape)} and {tuple(teacher_ids.shape)}")  # fmt: skip
+    if logits.shape[-1] > 1 << 19:
+        raise ValueError(f"{what}: a vocabulary of at most {1 << 19}, got {logits.shape[-1]}")
     if not temperature > 0:
         raise ValueError(f"{what}: the temperature must be positive, got {temperature}")
     if reduction not in ("none", "sum", "mean"):
@@ -439,7 +449,7 @@ def topk_distill_loss(logits: Tensor, teacher_ids: Tensor, teacher_logits: Tenso
         return _TopkDistill.apply(logits, ids, top, float(temperature), row_weight, factor, reduced)
     call = _Distill(logits, ids, top, float(temperature), row_weight, factor)
     total = torch.empty((), device=logits.device, dtype=torch.float32) if reduced else None
-    losses = call.forward(None, total, None)
+    losses = call.forward(torch.empty((rows, 2), device=logits.device, dtype=torch.float32), total, None)
     return total if reduced else losses
 
 

@@ -68,20 +68,21 @@ int ebr_expert_combine(int dtype, int weight_dtype, int64_t T, int64_t K, int64_
  *   total = factor * sum over n of losses[n],
  *   grad[n, j] = factor * u_n * w_n * tau * (q_j - sum of p_k with id_k = j),
  * entries with p_k = 0 adding nothing. A row without entries, or with w_n = 0, has loss 0 and gradient 0 whatever its
- * logits hold, and its logits are not read. 1 <= K <= 4096, 1 <= V < 2^31, tau > 0.
+ * logits hold. 1 <= K <= 1024, 1 <= V <= 2^19, tau > 0.
  *
  * ebr_topk_distill: losses [N] float32; stats [N, 2] float32 (each row's largest logit and its sum of
- * exp((s - largest) / tau)), or NULL; total: one float32 (a sum in a fixed order), or NULL; grad [N, V] of type dtype,
- * contiguous, made with u_n = 1, or NULL.
+ * exp((s - largest) / tau); 0 and infinity for a row that does not count); total: one float32 (a sum in a fixed order), or NULL; grad [N, V] of type dtype
+ * (row stride grad_stride, unit column stride), made with u_n = 1, or NULL.
  * ebr_topk_distill_grad: grad from the forward's stats, u_n = upstream[upstream_stride * n] (stride 0 or 1). With
  * unless_one != 0 and stride 0, nothing is written where upstream[0] is exactly 1: grad was made with it already. */
 int ebr_topk_distill(int dtype, int id_type, int top_dtype, int64_t N, int64_t V, int64_t K, double tau, double factor,
                      const void* logits, int64_t logits_stride, const void* top_ids, const void* top_logits,
-                     const float* row_weight, float* losses, float* stats, float* total, void* grad, void* stream);
+                     const float* row_weight, float* losses, float* stats, float* total, void* grad, int64_t grad_stride,
+                     void* stream);
 int ebr_topk_distill_grad(int dtype, int id_type, int top_dtype, int64_t N, int64_t V, int64_t K, double tau,
                           double factor, const void* logits, int64_t logits_stride, const void* top_ids,
                           const void* top_logits, const float* row_weight, const float* stats, const float* upstream,
-                          int64_t upstream_stride, int unless_one, void* grad, void* stream);
+                          int64_t upstream_stride, int unless_one, void* grad, int64_t grad_stride, void* stream);
 
 #ifdef __cplusplus
 }
