@@ -8,6 +8,8 @@
 // under 62,208 tokens (runs of thousands) and one of 131,072 rows (runs of one or two) take the same path.
 #pragma once
 
+#include <type_traits>
+
 #include "key_sort.cuh"
 #include "layers.cuh"
 
@@ -16,15 +18,86 @@ namespace embed {
 
 using keysort::IdSource;
 
+// kBytes bytes as one access.
+template <int kBytes>
+struct Word;
+template <>
+struct Word<2> {
+  using type = unsigned short;
+};
+template <>
+struct Word<4> {
+  using type = unsigned;
+};
+template <>
+struct Word<8> {
+  using type = uint2;
+};
+template <>
+struct Word<16> {
+  using type = uint4;
+};
+
+// V elements of T as they are in memory (at most 16 bytes), and as floats. The 16-bit types are converted two at a time
+// from whole words.
+template <typename T, int V>
+struct Raw {
+  using W = typename Word<V * sizeof(T)>::type;
+  W w = {};
+  __device__ __forceinline__ void load(const T* p) { w = *reinterpret_cast<const W*>(p); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<W*>(p) = w; }
+  __device__ __forceinline__ void widen(float (&v)[V]) const {
+    if constexpr (sizeof(T) == 4) {
+      const float* f = reinterpret_cast<const float*>(&w);
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] = f[i];
+    } else if constexpr (V == 1) {
+      v[0] = Elem<T>::load(reinterpret_cast<const T*>(&w));
+    } else {
+      const unsigned* u = reinterpret_cast<const unsigned*>(&w);
+#pragma unroll
+      for (int i = 0; i < V; i += 2) {
+        if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+          v[i] = __uint_as_float(u[i / 2] << 16);
+          v[i + 1] = __uint_as_float(u[i / 2] & 0xffff0000u);
+        } else {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[i / 2]));
+          v[i] = f.x;
+          v[i + 1] = f.y;
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void narrow(const float (&v)[V]) {
+    if constexpr (sizeof(T) == 4) {
+      float* f = reinterpret_cast<float*>(&w);
+#pragma unroll
+      for (int i = 0; i < V; ++i) f[i] = v[i];
+    } else if constexpr (V == 1) {
+      *reinterpret_cast<T*>(&w) = Elem<T>::to(v[0]);
+    } else {
+      unsigned* u = reinterpret_cast<unsigned*>(&w);
+#pragma unroll
+      for (int i = 0; i < V; i += 2) {
+        const float2 f = make_float2(v[i], v[i + 1]);
+        if constexpr (std::is_same_v<T, __nv_bfloat16>)
+          *reinterpret_cast<__nv_bfloat162*>(&u[i / 2]) = __float22bfloat162_rn(f);
+        else
+          *reinterpret_cast<__half2*>(&u[i / 2]) = __float22half2_rn(f);
+      }
+    }
+  }
+};
+
 // V consecutive elements as floats, in accesses of at most 16 bytes.
 template <typename T, int V>
 __device__ __forceinline__ void load_f(const T* p, float (&out)[V]) {
   constexpr int kStep = V * sizeof(T) > 16 ? 16 / sizeof(T) : V;
 #pragma unroll
   for (int s = 0; s < V; s += kStep) {
-    const layers::Pack<T, kStep> pk = *reinterpret_cast<const layers::Pack<T, kStep>*>(p + s);
-#pragma unroll
-    for (int i = 0; i < kStep; ++i) out[s + i] = Elem<T>::load(&pk.e[i]);
+    Raw<T, kStep> r;
+    r.load(p + s);
+    r.widen(*reinterpret_cast<float(*)[kStep]>(out + s));
   }
 }
 
@@ -33,49 +106,55 @@ __device__ __forceinline__ void store_f(T* p, const float (&in)[V]) {
   constexpr int kStep = V * sizeof(T) > 16 ? 16 / sizeof(T) : V;
 #pragma unroll
   for (int s = 0; s < V; s += kStep) {
-    layers::Pack<T, kStep> pk;
-#pragma unroll
-    for (int i = 0; i < kStep; ++i) pk.e[i] = Elem<T>::to(in[s + i]);
-    *reinterpret_cast<layers::Pack<T, kStep>*>(p + s) = pk;
+    Raw<T, kStep> r;
+    r.narrow(*reinterpret_cast<const float(*)[kStep]>(in + s));
+    r.store(p + s);
   }
 }
 
 // ------------------------------------------------------------------------------------------------ lookup
 
-// A warp writes up to 32 consecutive tokens' parts of 32 vectors of columns (blockIdx.y picks them): its lanes read the
-// ids at once, and kLookupAhead rows are in flight, so that the chain id -> row -> store is paid once for many rows.
-constexpr int kLookupWarps = 8, kLookupAhead = 4;
+// A warp writes up to 32 consecutive tokens' parts of kU * 32 vectors of columns (blockIdx.y picks them): its lanes read
+// the ids at once, and kLookupAhead / kU rows are in flight, so that the chain id -> row -> store is paid once for many
+// rows. Whole rows by one warp where they fit: neighbouring rows are then written as one stretch.
+constexpr int kLookupWarps = 4, kLookupAhead = 4;
 
-template <typename TW, typename TO, int V>
+template <typename TW, typename TO, int V, int kU>
 __global__ void __launch_bounds__(kLookupWarps * 32) lookup_kernel(IdSource src, int64_t n, int64_t C, float scale,
                                                                    const TW* __restrict__ w, int64_t w_stride,
                                                                    TO* __restrict__ out, int per_warp) {
+  constexpr int kRows = kLookupAhead / kU;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t c = (static_cast<int64_t>(blockIdx.y) * 32 + lane) * V;
-  const bool live = c < C;
+  const int64_t c0 = (static_cast<int64_t>(blockIdx.y) * kU * 32 + lane) * V;
   const int64_t t0 = (static_cast<int64_t>(blockIdx.x) * kLookupWarps + warp) * per_warp;
   const int tokens = static_cast<int>(min(static_cast<int64_t>(per_warp), n - t0));  // may be <= 0
   const int my_id = lane < tokens ? src.key(t0 + lane) : src.range;
-  TO* dst = out + t0 * C + c;
-  for (int j0 = 0; j0 < tokens; j0 += kLookupAhead) {
-    float v[kLookupAhead][V];
+  TO* dst = out + t0 * C + c0;
+  for (int j0 = 0; j0 < tokens; j0 += kRows) {
+    float v[kRows][kU][V];
 #pragma unroll
-    for (int u = 0; u < kLookupAhead; ++u) {
-      const int id = __shfl_sync(0xffffffffu, my_id, (j0 + u) & 31);
-      if (id < src.range && live && j0 + u < tokens) {
-        load_f<TW, V>(w + id * w_stride + c, v[u]);
-      } else {
+    for (int r = 0; r < kRows; ++r) {
+      const int id = __shfl_sync(0xffffffffu, my_id, (j0 + r) & 31);
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[u][i] = 0.f;
+      for (int u = 0; u < kU; ++u) {
+        const int64_t c = c0 + u * 32 * V;
+        if (id < src.range && c < C && j0 + r < tokens) {
+          load_f<TW, V>(w + id * w_stride + c, v[r][u]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < V; ++i) v[r][u][i] = 0.f;
+        }
       }
     }
 #pragma unroll
-    for (int u = 0; u < kLookupAhead; ++u) {
-      if (j0 + u >= tokens || !live) continue;
+    for (int r = 0; r < kRows; ++r)
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[u][i] *= scale;
-      store_f<TO, V>(dst + (j0 + u) * C, v[u]);
-    }
+      for (int u = 0; u < kU; ++u) {
+        if (j0 + r >= tokens || c0 + u * 32 * V >= C) continue;
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[r][u][i] *= scale;
+        store_f<TO, V>(dst + (j0 + r) * C + u * 32 * V, v[r][u]);
+      }
   }
 }
 
@@ -93,7 +172,6 @@ __global__ void __launch_bounds__(kGradWarps * 32) grad_chunk_kernel(int n, int 
                                                                      float scale, TW* __restrict__ dw,
                                                                      float* __restrict__ part) {
   constexpr int kAhead = 8;  // rows in flight
-  using Raw = layers::Pack<TG, V>;
   const int lane = threadIdx.x & 31;
   const int64_t chunk = static_cast<int64_t>(blockIdx.x) * kGradWarps + (threadIdx.x >> 5);
   const int64_t begin = chunk * R;
@@ -107,9 +185,11 @@ __global__ void __launch_bounds__(kGradWarps * 32) grad_chunk_kernel(int n, int 
   float acc[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) acc[i] = 0.f;
-  auto add = [&](const Raw& r) {
+  auto add = [&](const Raw<TG, V>& r) {
+    float v[V];
+    r.widen(v);
 #pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] += Elem<TG>::load(&r.e[i]);
+    for (int i = 0; i < V; ++i) acc[i] += v[i];
   };
   auto flush = [&](bool goes_on) {
     if (live) {
@@ -131,12 +211,11 @@ __global__ void __launch_bounds__(kGradWarps * 32) grad_chunk_kernel(int n, int 
     const int my_row = lane < rows ? order[r0 + lane] : 0;
     const int valid = __popc(__ballot_sync(0xffffffffu, my_key < range));  // the first ones: the keys are sorted
     for (int j0 = 0; j0 < valid; j0 += kAhead) {
-      Raw v[kAhead];
+      Raw<TG, V> v[kAhead];
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
         const int64_t row = __shfl_sync(0xffffffffu, my_row, (j0 + u) & 31);
-        v[u] = {};
-        if (j0 + u < valid && live) v[u] = *reinterpret_cast<const Raw*>(g + row * g_stride + c);
+        if (j0 + u < valid && live) v[u].load(g + row * g_stride + c);
       }
       const int last = __shfl_sync(0xffffffffu, my_key, min(j0 + kAhead, valid) - 1);
       if (last == cur) {  // one run: the rows past `valid` add zeros
@@ -225,11 +304,13 @@ __global__ void __launch_bounds__(kJoinWarps * 32) grad_join_kernel(int n, int r
       if (id >= range || key[end] != id || (begin > 0 && key[begin - 1] == id)) id = -1;
     }
     if (id >= 0) {  // the last chunk that starts with this id: the keys at the chunks' starts are in order
+      // [lo, hi]; 32 probes at a time
       int64_t lo = chunk + 1, hi = chunks - 1;
-      if (lo + kJoinShort <= hi && key[(lo + kJoinShort) * R] != id) hi = lo + kJoinShort;
       while (lo < hi) {
-        const int64_t mid = (lo + hi + 1) / 2;
-        if (key[mid * R] == id) lo = mid; else hi = mid - 1;
+        const int64_t gap = (hi - lo + 31) / 32, at = min(hi, lo + (lane + 1) * gap);
+        const int hits = __popc(__ballot_sync(0xffffffffu, key[at * R] == id));  // the first ones
+        hi = min(hi, lo + (hits + 1) * gap - 1);
+        lo = min(hi, lo + hits * gap);
       }
       last = lo;
       if (last - chunk < kJoinShort) {

@@ -62,10 +62,14 @@ int access_width(int most, int64_t C, std::initializer_list<Rows> rows) {
   return v;
 }
 
-template <typename Fn>
+// Vectors of a row that a warp of the expert kernels has in flight: two of the widest, eight of single elements.
+constexpr int unroll_of(int v) { return v >= 8 ? 2 : v == 4 ? 4 : 8; }
+
+template <int kMost, typename Fn>
 int with_width(int v, Fn&& fn) {
   switch (v) {
-    case 8: return fn(std::integral_constant<int, 8>{});
+    case 8:
+      if constexpr (kMost >= 8) return fn(std::integral_constant<int, 8>{});
     case 4: return fn(std::integral_constant<int, 4>{});
     case 2: return fn(std::integral_constant<int, 2>{});
     default: return fn(std::integral_constant<int, 1>{});
@@ -74,8 +78,19 @@ int with_width(int v, Fn&& fn) {
 
 // ------------------------------------------------------------------------------------------------ sort
 
-// Keys that one cluster of 16 CTAs ranks in registers.
+// Keys that one cluster of 16 CTAs ranks in registers, and those up to which it is used even where nothing runs beside
+// it: 18,006 slots take 8.7 us in a cluster; 124,416 take 15.6 there and XX in two kernels over the whole GPU.
 constexpr int64_t kClusterKeys = 16 * int64_t{ebr::keysort::kSortThreads} * 16;
+constexpr int64_t kClusterAlone = 32 * 1024;
+
+// Bytes of zeros from which the sort in one cluster hides behind the zeroing, and up to which the sort's own blocks write
+// them.
+constexpr int64_t kHidingBytes = 64 << 20;
+constexpr int64_t kSmallZeroBytes = 1 << 20;
+
+bool sort_in_cluster(int64_t n, int64_t zero_bytes) {
+  return n <= kClusterAlone || (n <= kClusterKeys && zero_bytes >= kHidingBytes);
+}
 
 int digit_passes(int64_t range) {  // keys in [0, range]
   int bits = 1;
@@ -89,18 +104,23 @@ int digit_bits(int64_t range, int passes) {
   return (bits + passes - 1) / passes;
 }
 
-int64_t sort_tiles(int64_t n) { return (n + ebr::keysort::kTile - 1) / ebr::keysort::kTile; }
+// Items per thread and tiles of the whole-grid sort.
+int sort_items(int64_t n) { return n <= int64_t{2} * ebr::keysort::kSortThreads * ebr::keysort::kMaxTiles ? 2 : 8; }
+int64_t sort_tiles(int64_t n) {
+  const int64_t tile = static_cast<int64_t>(sort_items(n)) * ebr::keysort::kSortThreads;
+  return (n + tile - 1) / tile;
+}
 
 // Scratch of a sort: two (key, position) arrays where there is output, and the whole-grid path's counts.
 size_t sort_scratch(int64_t n, int64_t digits, int passes, bool route) {
   size_t b = 0;
   if (!route) b += (passes > 1 ? 4 : 2) * round16(static_cast<size_t>(n) * 4);
-  if (n > kClusterKeys) b += round16(static_cast<size_t>(digits) * sort_tiles(n) * 4) + round16(digits * 4);
+  if (n > kClusterAlone) b += round16(static_cast<size_t>(digits) * sort_tiles(n) * 4) + round16(digits * 4);
   return b;
 }
 
 template <int kItems>
-int launch_cluster_sort(int device, const ClusterSort& a, int ctas, int bits, int fill_clusters, cudaStream_t st) {
+int launch_cluster_sort(int device, const ClusterSort& a, int ctas, int bits, cudaStream_t st) {
   auto* kernel = ebr::keysort::cluster_sort_kernel<kItems>;
   static std::atomic<bool> ready[kMaxDevices];
   if (device >= kMaxDevices || !ready[device].load()) {
@@ -112,7 +132,7 @@ int launch_cluster_sort(int device, const ClusterSort& a, int ctas, int bits, in
     if (device < kMaxDevices) ready[device].store(true);
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(ctas * (1 + fill_clusters)));
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
   cfg.blockDim = dim3(ebr::keysort::kSortThreads);
   cfg.dynamicSmemBytes = ebr::keysort::cluster_sort_smem(bits);
   cfg.stream = st;
@@ -126,10 +146,52 @@ int launch_cluster_sort(int device, const ClusterSort& a, int ctas, int bits, in
   return check_launch("cluster sort");
 }
 
+// Zeros, beside the cluster sort that was launched before where `beside`.
+int launch_zero(void* p, int64_t bytes, bool beside, cudaStream_t st) {
+  if (bytes == 0) return EBR_OK;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>((bytes + ebr::keysort::kZeroPiece - 1) / ebr::keysort::kZeroPiece));
+  cfg.blockDim = dim3(1024);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = beside ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, ebr::keysort::zero_kernel, static_cast<char*>(p), bytes);
+  if (e != cudaSuccess) return cuda_error(e, "zeroing");
+  return check_launch("zeroing");
+}
+
+template <int kItems>
+int launch_grid_sort(GridSort& g, const ebr::keysort::Pass* pass, int passes, cudaStream_t st) {
+  const size_t smem = ebr::keysort::grid_place_smem(g.digits);
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(ebr::keysort::grid_place_kernel<kItems>,
+                                               cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    if (e != cudaSuccess) return cuda_error(e, "sort attributes");
+  }
+  g.scanned = g.tiles > ebr::keysort::kMaxTiles;
+  for (int p = 0; p < passes; ++p) {
+    g.pass = pass[p];
+    ebr::keysort::grid_count_kernel<kItems><<<g.tiles, ebr::keysort::kSortThreads, 0, st>>>(g);
+    int rc = check_launch("sort count");
+    if (rc != EBR_OK) return rc;
+    if (g.scanned) {
+      ebr::keysort::grid_scan_kernel<<<g.digits, ebr::keysort::kSortThreads, 0, st>>>(g);
+      if ((rc = check_launch("sort scan")) != EBR_OK) return rc;
+    }
+    ebr::keysort::grid_place_kernel<kItems><<<g.tiles, ebr::keysort::kSortThreads, smem, st>>>(g);
+    if ((rc = check_launch("sort place")) != EBR_OK) return rc;
+  }
+  return EBR_OK;
+}
+
 // Sort n keys of [0, range]; digits: of one pass. For a route (route.row_of set) there is one pass, else the sorted keys
-// and positions are at *key / *order in the scratch. `fill` bytes are zeroed beside or before the sort.
+// and positions are at *key / *order in the scratch. `zero_bytes` at `zero` (16-byte aligned) are zeroed beside or before
+// the sort.
 int run_sort(int device, IdSource src, int64_t n, int passes, int bits, const ebr::keysort::RouteOut& route,
-             void* scratch, int** key, int** order, void* fill, int64_t fill_bytes, cudaStream_t st) {
+             void* scratch, int** key, int** order, void* zero, int64_t zero_bytes, cudaStream_t st) {
   char* at = static_cast<char*>(scratch);
   auto take = [&](size_t bytes) {
     char* p = at;
@@ -158,32 +220,33 @@ int run_sort(int device, IdSource src, int64_t n, int passes, int bits, const eb
   } else {
     pass[0].bits = bits;
   }
-  if (n <= kClusterKeys) {
+  ebr::keysort::SmallZero small = {nullptr, 0};
+  if (zero_bytes <= kSmallZeroBytes) {
+    small = {static_cast<char*>(zero), zero_bytes};
+    zero_bytes = 0;
+  }
+  if (sort_in_cluster(n, zero_bytes)) {
     ClusterSort a = {};
+    a.zero = small;
     a.src = src;
     a.n = n;
     a.passes = passes;
     for (int p = 0; p < 3; ++p) a.pass[p] = pass[p];
     a.route = route;
-    a.fill = fill;
-    a.fill_bytes = fill_bytes;
     int ctas = 1;
     while (ctas < 16 && static_cast<int64_t>(ctas) * ebr::keysort::kSortThreads < n) ctas *= 2;
     const int64_t per_thread = ((n + ctas - 1) / ctas + ebr::keysort::kSortThreads - 1) / ebr::keysort::kSortThreads;
-    // zeroing CTAs: one for 128 KB, whole clusters; many, so that the SMs that the sort leaves free even out
-    const int64_t fill_ctas = fill ? std::min<int64_t>((fill_bytes + 131071) / 131072, 1 << 20) : 0;
-    const int fill_clusters = static_cast<int>((fill_ctas + ctas - 1) / ctas);
-    if (per_thread <= 1) return launch_cluster_sort<1>(device, a, ctas, bits, fill_clusters, st);
-    if (per_thread <= 2) return launch_cluster_sort<2>(device, a, ctas, bits, fill_clusters, st);
-    if (per_thread <= 4) return launch_cluster_sort<4>(device, a, ctas, bits, fill_clusters, st);
-    if (per_thread <= 8) return launch_cluster_sort<8>(device, a, ctas, bits, fill_clusters, st);
-    return launch_cluster_sort<16>(device, a, ctas, bits, fill_clusters, st);
+    const int rc = per_thread <= 1   ? launch_cluster_sort<1>(device, a, ctas, bits, st)
+                   : per_thread <= 2 ? launch_cluster_sort<2>(device, a, ctas, bits, st)
+                   : per_thread <= 4 ? launch_cluster_sort<4>(device, a, ctas, bits, st)
+                   : per_thread <= 8 ? launch_cluster_sort<8>(device, a, ctas, bits, st)
+                                     : launch_cluster_sort<16>(device, a, ctas, bits, st);
+    return rc != EBR_OK ? rc : launch_zero(zero, zero_bytes, true, st);
   }
-  if (fill && fill_bytes) {
-    const cudaError_t e = cudaMemsetAsync(fill, 0, static_cast<size_t>(fill_bytes), st);
-    if (e != cudaSuccess) return cuda_error(e, "zeroing");
-  }
+  const int rc = launch_zero(zero, zero_bytes, false, st);
+  if (rc != EBR_OK) return rc;
   GridSort g = {};
+  g.zero = small;
   g.src = src;
   g.n = n;
   g.digits = is_route ? route.experts : 1 << bits;
@@ -191,23 +254,7 @@ int run_sort(int device, IdSource src, int64_t n, int passes, int bits, const eb
   g.counts = take(static_cast<size_t>(g.digits) * g.tiles * 4);
   g.totals = take(static_cast<size_t>(g.digits) * 4);
   g.route = route;
-  const size_t smem = ebr::keysort::grid_place_smem(g.digits);
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(ebr::keysort::grid_place_kernel,
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (e != cudaSuccess) return cuda_error(e, "sort attributes");
-  }
-  for (int p = 0; p < passes; ++p) {
-    g.pass = pass[p];
-    ebr::keysort::grid_count_kernel<<<g.tiles, ebr::keysort::kSortThreads, g.digits * 4, st>>>(g);
-    int rc = check_launch("sort count");
-    if (rc != EBR_OK) return rc;
-    ebr::keysort::grid_scan_kernel<<<g.digits, ebr::keysort::kSortThreads, 0, st>>>(g);
-    if ((rc = check_launch("sort scan")) != EBR_OK) return rc;
-    ebr::keysort::grid_place_kernel<<<g.tiles, ebr::keysort::kSortThreads, smem, st>>>(g);
-    if ((rc = check_launch("sort place")) != EBR_OK) return rc;
-  }
-  return EBR_OK;
+  return sort_items(n) == 2 ? launch_grid_sort<2>(g, pass, passes, st) : launch_grid_sort<8>(g, pass, passes, st);
 }
 
 // ------------------------------------------------------------------------------------------------ embedding
@@ -222,11 +269,12 @@ int check_embedding(int id_type, int64_t n, int64_t V, int64_t C, int64_t stride
   return EBR_OK;
 }
 
-// Rows of a chunk of the gradient, 8 to 256: some 4,000 warps' worth of chunks.
+// Rows of a chunk of the gradient, 8 to 256: some 3,000 warps' worth of chunks (62,208 board tokens of 512 columns: the
+// whole gradient takes 35 us with 64 rows, 42 with 32, which leave twice the partial sums to join).
 int64_t grad_chunk_rows(int64_t n, int64_t C) {
   const int64_t blocks = (C + 255) / 256;
   int64_t r = 8;
-  while (r < 256 && n * blocks / r > 6000) r *= 2;
+  while (r < 256 && n * blocks / r > 3000) r *= 2;
   return r;
 }
 
@@ -394,18 +442,19 @@ int ebr_scaled_embedding(int w_dtype, int out_dtype, int id_type, int64_t n, int
   return with_types(w_dtype, out_dtype, [&](auto* wt, auto* ot) -> int {
     using TW = std::remove_pointer_t<decltype(wt)>;
     using TO = std::remove_pointer_t<decltype(ot)>;
-    const int most = sizeof(TW) == 4 && sizeof(TO) == 4 ? 4 : 8;
-    const int v = access_width(most, C, {{w, w_stride, int(sizeof(TW))}, {out, C, int(sizeof(TO))}});
-    return with_width(v, [&](auto vc) -> int {
+    constexpr int kMost = sizeof(TW) == 4 && sizeof(TO) == 4 ? 4 : 8;
+    const int v = access_width(kMost, C, {{w, w_stride, int(sizeof(TW))}, {out, C, int(sizeof(TO))}});
+    return with_width<kMost>(v, [&](auto vc) -> int {
       constexpr int V_ = decltype(vc)::value;
       using namespace ebr::embed;
-      const int64_t cols = (C + 32 * V_ - 1) / (32 * V_);
+      constexpr int kU = V_ >= 4 ? 1 : 4;  // vectors of a row in flight: narrow ones need more
+      const int64_t cols = (C + kU * 32 * V_ - 1) / (kU * 32 * V_);
       if (cols > 65535) return set_error(EBR_ERR_SHAPE, "scaled_embedding: row too long%s%s");
       // as many tokens to a warp (up to 32) as leave some 24 warps for each SM
       int per_warp = 1;
       while (per_warp < 32 && n * cols / per_warp > 24 * static_cast<int64_t>(sm_count(device))) per_warp *= 2;
       const int64_t blocks = (n + per_warp * kLookupWarps - 1) / (per_warp * kLookupWarps);
-      lookup_kernel<TW, TO, V_><<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(cols)), kLookupWarps * 32,
+      lookup_kernel<TW, TO, V_, kU><<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(cols)), kLookupWarps * 32,
                                   0, st>>>(IdSource{ids, id_type == EBR_INT64, static_cast<int>(V)}, n, C,
                                            static_cast<float>(scale), static_cast<const TW*>(w), w_stride,
                                            static_cast<TO*>(out), per_warp);
@@ -439,6 +488,7 @@ int ebr_scaled_embedding_grad(int g_dtype, int w_dtype, int id_type, int64_t n, 
     return e == cudaSuccess ? EBR_OK : cuda_error(e, "scaled_embedding_grad");
   }
   if (!ids || !g) return set_error(EBR_ERR_NULL, "scaled_embedding_grad: NULL pointer%s%s");
+  if (!aligned16(dw)) return set_error(EBR_ERR_STRIDE, "scaled_embedding_grad: dW must be 16-byte aligned%s%s");
   if (!scratch || !aligned16(scratch) || scratch_bytes < ebr_scaled_embedding_grad_scratch_bytes(n, V, C))
     return set_error(EBR_ERR_SCRATCH, "scaled_embedding_grad: scratch too small or unaligned%s%s");
   if ((rc = check_device(&device)) != EBR_OK) return rc;
@@ -455,9 +505,9 @@ int ebr_scaled_embedding_grad(int g_dtype, int w_dtype, int id_type, int64_t n, 
     using TG = std::remove_pointer_t<decltype(gt)>;
     using TW = std::remove_pointer_t<decltype(wt)>;
     using namespace ebr::embed;
-    const int most = sizeof(TG) == 4 ? 4 : 8;
-    const int v = access_width(most, C, {{g, g_stride, int(sizeof(TG))}, {dw, C, int(sizeof(TW))}, {part, C, 4}});
-    int r = with_width(v, [&](auto vc) -> int {
+    constexpr int kMost = static_cast<int>(16 / sizeof(TG));
+    const int v = access_width(kMost, C, {{g, g_stride, int(sizeof(TG))}, {dw, C, int(sizeof(TW))}, {part, C, 4}});
+    int r = with_width<kMost>(v, [&](auto vc) -> int {
       constexpr int V_ = decltype(vc)::value;
       const int64_t cols = (C + 32 * V_ - 1) / (32 * V_);
       if (cols > 65535) return set_error(EBR_ERR_SHAPE, "scaled_embedding_grad: row too long%s%s");
@@ -477,6 +527,16 @@ int ebr_scaled_embedding_grad(int g_dtype, int w_dtype, int id_type, int64_t n, 
     return check_launch("scaled_embedding_grad join");
   });
 }
+
+}  // extern "C"
+
+namespace {
+int64_t expert_blocks(int device, int64_t T) {
+  return std::min<int64_t>((T + ebr::experts::kWarps - 1) / ebr::experts::kWarps, 16 * int64_t{sm_count(device)});
+}
+}  // namespace
+
+extern "C" {
 
 size_t ebr_expert_route_scratch_bytes(int64_t T, int64_t K, int64_t E) {
   if (T <= 0 || K <= 0 || E < 1 || E > kMaxExperts || T >= kMaxSortKeys || K >= kMaxSortKeys || T * K >= kMaxSortKeys)
@@ -536,16 +596,16 @@ int ebr_expert_scatter(int dtype, int weight_dtype, int64_t T, int64_t K, int64_
     if constexpr (std::is_same_v<T_, double>) {
       return EBR_ERR_DTYPE;
     } else {
-      const int size = sizeof(T_);
-      const int v = access_width(16 / size, C, {{x, x_stride, size}, {rows_in, C, size}, {rows_out, C, size}});
-      return with_width(v, [&](auto vc) -> int {
+      constexpr int size = sizeof(T_), kMost = 16 / size;
+      const int v = access_width(kMost, C, {{x, x_stride, size}, {rows_in, C, size}, {rows_out, C, size}});
+      return with_width<kMost>(v, [&](auto vc) -> int {
         constexpr int V_ = decltype(vc)::value;
         auto launch = [&](auto* wtag, auto with_dots) -> int {
           using TW = std::remove_pointer_t<decltype(wtag)>;
           using namespace ebr::experts;
-          const int64_t tb = (T + kWarps - 1) / kWarps;
+          const int64_t tb = expert_blocks(device, T);
           const int64_t zb = rows_out ? (rows + kZeroRows - 1) / kZeroRows : 0;
-          scatter_kernel<T_, TW, V_, decltype(with_dots)::value><<<static_cast<unsigned>(tb + zb), kWarps * 32, 0, st>>>(
+          scatter_kernel<T_, TW, V_, unroll_of(V_), decltype(with_dots)::value><<<static_cast<unsigned>(tb + zb), kWarps * 32, 0, st>>>(
               T, static_cast<int>(K), C, rows, static_cast<const T_*>(x), x_stride, row_of, slot_of,
               static_cast<const TW*>(weights), static_cast<const T_*>(rows_in), static_cast<T_*>(rows_out),
               static_cast<TW*>(dots), static_cast<int>(tb));
@@ -580,14 +640,14 @@ int ebr_expert_combine(int dtype, int weight_dtype, int64_t T, int64_t K, int64_
     if constexpr (std::is_same_v<T_, double>) {
       return EBR_ERR_DTYPE;
     } else {
-      const int size = sizeof(T_);
-      const int v = access_width(16 / size, C, {{rows_in, rows_stride, size}, {y, C, size}});
-      return with_width(v, [&](auto vc) -> int {
+      constexpr int size = sizeof(T_), kMost = 16 / size;
+      const int v = access_width(kMost, C, {{rows_in, rows_stride, size}, {y, C, size}});
+      return with_width<kMost>(v, [&](auto vc) -> int {
         constexpr int V_ = decltype(vc)::value;
         auto launch = [&](auto* wtag) -> int {
           using TW = std::remove_pointer_t<decltype(wtag)>;
           using namespace ebr::experts;
-          combine_kernel<T_, TW, V_><<<static_cast<unsigned>((T + kWarps - 1) / kWarps), kWarps * 32, 0, st>>>(
+          combine_kernel<T_, TW, V_, unroll_of(V_)><<<static_cast<unsigned>(expert_blocks(device, T)), kWarps * 32, 0, st>>>(
               T, static_cast<int>(K), C, static_cast<const T_*>(rows_in), rows_stride, row_of,
               static_cast<const TW*>(weights), static_cast<T_*>(y));
           return check_launch("expert_combine");

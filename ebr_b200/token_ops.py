@@ -15,8 +15,7 @@ An id outside its range is a padding id everywhere: a zero row, no expert, no en
 
 from __future__ import annotations
 
-from dataclasses import dataclass
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -46,12 +45,14 @@ def _require(t: Tensor, what: str, name: str, types: dict, device: Optional[torc
 
 
 def _call(what: str, device: torch.device, fn, *args) -> None:
-    """``fn(*args, stream)`` on ``device``'s current stream (the C ABI launches on the current device)."""
-    if device.index == torch.cuda.current_device():
-        status = fn(*args, torch.cuda.current_stream().cuda_stream)
+    """``fn(*args, stream)`` on ``device``'s current stream (the C ABI launches on the current device). The raw stream
+    handle is asked for directly: a ``torch.cuda.Stream`` object costs as much host time as the launch."""
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            status = fn(*args, torch.cuda.current_stream().cuda_stream)
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     if status:
         _native.check(status, what)
 
@@ -66,8 +67,8 @@ def _row_view(t: Tensor) -> Tuple[Tensor, int]:
     return t.contiguous(), c
 
 
-def _scratch(nbytes: int, device: torch.device) -> Optional[Tensor]:
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+def _scratch(nbytes: int, like: Tensor) -> Optional[Tensor]:
+    return like.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
 
 
 def _ptr(t: Optional[Tensor]):
@@ -80,7 +81,7 @@ def _ptr(t: Optional[Tensor]):
 def _lookup(tokens: Tensor, weight: Tensor, scale: float, dtype: torch.dtype) -> Tensor:
     weight, stride = _row_view(weight)
     v, c = weight.shape
-    out = torch.empty((*tokens.shape, c), device=weight.device, dtype=dtype)
+    out = weight.new_empty((*tokens.shape, c), dtype=dtype)
     _call("scaled_embedding", weight.device, _native.lib().ebr_scaled_embedding, _DTYPES[weight.dtype], _DTYPES[dtype],
           _IDS[tokens.dtype], tokens.numel(), v, c, scale, tokens.data_ptr(), weight.data_ptr(), stride,
           out.data_ptr())  # fmt: skip
@@ -90,10 +91,10 @@ def _lookup(tokens: Tensor, weight: Tensor, scale: float, dtype: torch.dtype) ->
 def _lookup_grad(tokens: Tensor, g: Tensor, scale: float, rows: int, dtype: torch.dtype) -> Tensor:
     g, stride = _row_view(g)
     n, c = tokens.numel(), g.shape[-1]
-    dw = torch.empty((rows, c), device=g.device, dtype=dtype)
+    dw = g.new_empty((rows, c), dtype=dtype)
     lib = _native.lib()
     nbytes = lib.ebr_scaled_embedding_grad_scratch_bytes(n, rows, c)
-    scratch = _scratch(nbytes, g.device)
+    scratch = _scratch(nbytes, g)
     _call("scaled_embedding_grad", g.device, lib.ebr_scaled_embedding_grad, _DTYPES[g.dtype], _DTYPES[dtype],
           _IDS[tokens.dtype], n, rows, c, scale, tokens.data_ptr(), g.data_ptr(), stride, dw.data_ptr(), _ptr(scratch),
           nbytes)  # fmt: skip
@@ -152,8 +153,7 @@ def scaled_embedding(tokens: Tensor, weight: Tensor, scale: float = 1.0, dtype: 
 # ---------------------------------------------------------------------------------------------------- experts
 
 
-@dataclass(frozen=True)
-class ExpertRoute:
+class ExpertRoute(NamedTuple):
     """Where each token's slots go (``expert_route``). ``row_of`` [*tokens, K]: the slot's row, -1 for a dropped one.
     ``slot_of`` [rows]: the row's slot (token * K + k), -1 for a row of no slot. ``offsets`` [experts + 1]: the first
     sorted position of each expert, counting every slot, so ``offsets[1:] - offsets[:-1]`` are the experts' loads; without
@@ -191,12 +191,12 @@ def expert_route(expert_ids: Tensor, experts: int, capacity: Optional[int] = Non
     ids, dev = expert_ids.contiguous(), expert_ids.device
     k, slots = ids.shape[-1], ids.numel()
     rows = slots if capacity is None else experts * capacity
-    row_of = torch.empty(ids.shape, dtype=torch.int32, device=dev)
-    slot_of = torch.empty(rows, dtype=torch.int32, device=dev)
-    offsets = torch.empty(experts + 1, dtype=torch.int32, device=dev)
+    row_of = ids.new_empty(ids.shape, dtype=torch.int32)
+    slot_of = ids.new_empty(rows, dtype=torch.int32)
+    offsets = ids.new_empty(experts + 1, dtype=torch.int32)
     lib = _native.lib()
     nbytes = lib.ebr_expert_route_scratch_bytes(slots // k, k, experts)
-    scratch = _scratch(nbytes, dev)
+    scratch = _scratch(nbytes, ids)
     _call("expert_route", dev, lib.ebr_expert_route, _IDS[ids.dtype], slots // k, k, experts, capacity or 0,
           ids.data_ptr(), row_of.data_ptr(), slot_of.data_ptr(), offsets.data_ptr(), _ptr(scratch), nbytes)  # fmt: skip
     return ExpertRoute(row_of, slot_of, offsets, experts, capacity)
@@ -217,11 +217,11 @@ def _scatter(x: Tensor, route: ExpertRoute, weights: Optional[Tensor], rows_in: 
     weights, code = _weight_args(weights, x)
     if weights is None and dots_dtype is not None:
         code = _DTYPES[dots_dtype]
-    out = torch.empty((route.rows, c), device=x.device, dtype=x.dtype) if want_rows else None
+    out = x.new_empty((route.rows, c)) if want_rows else None
     dots = None
     if rows_in is not None:
         rows_in = rows_in.to(x.dtype).contiguous()
-        dots = torch.empty(route.row_of.shape, device=x.device, dtype=torch.float32 if code == _native.FLOAT32 else x.dtype)
+        dots = x.new_empty(route.row_of.shape, dtype=torch.float32 if code == _native.FLOAT32 else x.dtype)
     _call("expert_scatter", x.device, _native.lib().ebr_expert_scatter, _DTYPES[x.dtype], code,
           route.row_of.numel() // route.top_k, route.top_k, c, route.rows, x.data_ptr(), stride, route.row_of.data_ptr(),
           route.slot_of.data_ptr(), _ptr(weights), _ptr(rows_in), _ptr(out), _ptr(dots))  # fmt: skip
@@ -232,7 +232,7 @@ def _combine(rows: Tensor, route: ExpertRoute, weights: Optional[Tensor]) -> Ten
     rows, stride = _row_view(rows)
     c = rows.shape[-1]
     weights, code = _weight_args(weights, rows)
-    y = torch.empty((*route.row_of.shape[:-1], c), device=rows.device, dtype=rows.dtype)
+    y = rows.new_empty((*route.row_of.shape[:-1], c))
     _call("expert_combine", rows.device, _native.lib().ebr_expert_combine, _DTYPES[rows.dtype], code,
           route.row_of.numel() // route.top_k, route.top_k, c, rows.data_ptr(), stride, route.row_of.data_ptr(),
           _ptr(weights), y.data_ptr())  # fmt: skip
@@ -334,44 +334,61 @@ def expert_combine(rows: Tensor, route: ExpertRoute, weights: Optional[Tensor] =
 # ---------------------------------------------------------------------------------------------------- distillation
 
 
-class _Distill:
-    """One call's arguments, laid out for the C ABI."""
+def _distill_args(view: Tensor, ids: Tensor, top: Tensor, tau: float, factor: float):
+    """The leading arguments that both entry points share."""
+    k = ids.shape[-1]
+    return (_DTYPES[view.dtype], _IDS[ids.dtype], _DTYPES[top.dtype], ids.numel() // k, view.shape[-1], k, tau, factor)
 
-    def __init__(self, logits: Tensor, ids: Tensor, top: Tensor, tau: float, row_weight: Optional[Tensor],
-                 factor: float) -> None:  # fmt: skip
-        self.shape = logits.shape
-        self.logits, self.stride = _row_view(logits)
-        self.ids, self.top, self.row_weight = ids, top, row_weight
-        self.rows, self.vocab, self.k = ids.numel() // ids.shape[-1], logits.shape[-1], ids.shape[-1]
-        self.tau, self.factor = tau, factor
 
-    def _args(self):
-        return (_DTYPES[self.logits.dtype], _IDS[self.ids.dtype], _DTYPES[self.top.dtype], self.rows, self.vocab, self.k,
-                self.tau, self.factor, self.logits.data_ptr(), self.stride, self.ids.data_ptr(), self.top.data_ptr(),
-                _ptr(self.row_weight))  # fmt: skip
+def _distill(logits: Tensor, ids: Tensor, top: Tensor, tau: float, row_weight: Optional[Tensor], factor: float,
+             total: bool, gradient: bool):  # fmt: skip
+    """(losses, total or None, stats, gradient or None): ``ebr_topk_distill``."""
+    view, stride = _row_view(logits)
+    rows = ids.numel() // ids.shape[-1]
+    losses = logits.new_empty(ids.shape[:-1], dtype=torch.float32)
+    stats = logits.new_empty((rows, 2), dtype=torch.float32)
+    total = logits.new_empty((), dtype=torch.float32) if total else None
+    grad, grad_stride = _distill_grad_buffer(view, stride) if gradient else (None, 0)
+    _call("topk_distill_loss", logits.device, _native.lib().ebr_topk_distill,
+          *_distill_args(view, ids, top, tau, factor), view.data_ptr(), stride, ids.data_ptr(),
+          top.data_ptr(), _ptr(row_weight), losses.data_ptr(), stats.data_ptr(), _ptr(total), _ptr(grad),
+          grad_stride)  # fmt: skip
+    return losses, total, stats, grad
 
-    def forward(self, stats: Tensor, total: Optional[Tensor], grad: Optional[Tensor]) -> Tensor:
-        dev = self.logits.device
-        losses = torch.empty(self.ids.shape[:-1], device=dev, dtype=torch.float32)
-        _call("topk_distill_loss", dev, _native.lib().ebr_topk_distill, *self._args(), losses.data_ptr(), stats.data_ptr(),
-              _ptr(total), _ptr(grad), self._grad_stride(grad))  # fmt: skip
-        return losses
 
-    def gradient(self, stats: Tensor, upstream: Tensor, grad: Tensor, unless_one: bool) -> None:
-        _call("topk_distill_loss", self.logits.device, _native.lib().ebr_topk_distill_grad, *self._args(),
-              stats.data_ptr(), upstream.data_ptr(), 0 if upstream.numel() == 1 and upstream.dim() == 0 else 1,
-              int(unless_one), grad.data_ptr(), self._grad_stride(grad))  # fmt: skip
+def _distill_gradient(logits: Tensor, ids: Tensor, top: Tensor, tau: float, row_weight: Optional[Tensor], factor: float,
+                      stats: Tensor, upstream: Tensor, made: Optional[Tensor]) -> Tensor:  # fmt: skip
+    """The gradient for ``upstream``, a scalar or one value per row: ``ebr_topk_distill_grad``. ``made``: the buffer that
+    the forward filled for an upstream of 1."""
+    view, stride = _row_view(logits)
+    if made is None:
+        grad, grad_stride = _distill_grad_buffer(view, stride)
+    else:
+        grad, grad_stride = made, _grad_stride(made)
+    if upstream.dtype != torch.float32:
+        upstream = upstream.float()
+    if upstream.dim() == 0 or not any(upstream.stride()):  # one value, or one value expanded over the rows
+        per_row = 0
+    else:
+        upstream, per_row = upstream.contiguous(), 1
+    _call("topk_distill_loss", logits.device, _native.lib().ebr_topk_distill_grad,
+          *_distill_args(view, ids, top, tau, factor), view.data_ptr(), stride, ids.data_ptr(),
+          top.data_ptr(), _ptr(row_weight), stats.data_ptr(), upstream.data_ptr(), per_row, int(made is not None),
+          grad.data_ptr(), grad_stride)  # fmt: skip
+    return grad
 
-    def new_grad(self) -> Tensor:
-        """The gradient's buffer: contiguous, or with the logits' row stride where they are a view of slightly longer
-        rows (a padded vocabulary), so that both rows start at the same place of a 16-byte word."""
-        s = self.logits
-        if self.vocab < self.stride <= self.vocab + 256 and s.dim() == 2:
-            return torch.empty_strided(s.shape, s.stride(), device=s.device, dtype=s.dtype)
-        return torch.empty(self.shape, device=s.device, dtype=s.dtype)
 
-    def _grad_stride(self, grad: Optional[Tensor]) -> int:
-        return self.vocab if grad is None or grad.is_contiguous() else grad.stride(0)
+def _distill_grad_buffer(view: Tensor, stride: int) -> Tuple[Tensor, int]:
+    """The gradient's buffer and row stride: contiguous, or with the logits' row stride where they are a view of slightly
+    longer rows (a padded vocabulary), so that both rows start at the same place of a 16-byte word."""
+    v = view.shape[-1]
+    if v < stride <= v + 256 and view.dim() == 2:
+        return torch.empty_strided(view.shape, view.stride(), device=view.device, dtype=view.dtype), stride
+    return view.new_empty(view.shape), v
+
+
+def _grad_stride(grad: Tensor) -> int:
+    return grad.shape[-1] if grad.is_contiguous() else grad.stride(0)
 
 
 class _TopkDistill(torch.autograd.Function):
@@ -382,29 +399,25 @@ class _TopkDistill(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, ids, top, tau, row_weight, factor, reduced):
-        call = _Distill(logits, ids, top, tau, row_weight, factor)
-        dev = logits.device
-        stats = torch.empty((call.rows, 2), device=dev, dtype=torch.float32)
+        losses, total, stats, ctx.made = _distill(logits, ids, top, tau, row_weight, factor, reduced, reduced)
         ctx.save_for_backward(logits, ids, top, row_weight, stats)
-        ctx.tau, ctx.factor, ctx.reduced, ctx.made = tau, factor, reduced, None
-        if not reduced:
-            return call.forward(stats, None, None)
-        total = torch.empty((), device=dev, dtype=torch.float32)
-        ctx.made = call.new_grad()
-        call.forward(stats, total, ctx.made)
-        return total
+        ctx.tau, ctx.factor = tau, factor
+        return total if reduced else losses
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, g: Tensor):
+        if torch.is_grad_enabled():
+            return _TopkDistill._backward_once(ctx, g)
+        return _TopkDistill._backward(ctx, g)
+
+    @staticmethod
+    def _backward(ctx, g: Tensor):
         logits, ids, top, row_weight, stats = ctx.saved_tensors
-        call = _Distill(logits, ids, top, ctx.tau, row_weight, ctx.factor)
-        grad, ctx.made = ctx.made, None
-        unless_one = grad is not None
-        if grad is None:
-            grad = call.new_grad()
-        call.gradient(stats, g.to(torch.float32).contiguous(), grad, unless_one)
+        made, ctx.made = ctx.made, None
+        grad = _distill_gradient(logits, ids, top, ctx.tau, row_weight, ctx.factor, stats, g, made)
         return grad, None, None, None, None, None, None
+
+    _backward_once = staticmethod(once_differentiable(_backward.__func__))
 
 
 def topk_distill_loss(logits: Tensor, teacher_ids: Tensor, teacher_logits: Tensor, temperature: float = 1.0, *,
@@ -447,9 +460,7 @@ def topk_distill_loss(logits: Tensor, teacher_ids: Tensor, teacher_logits: Tenso
     reduced = reduction != "none"
     if torch.is_grad_enabled() and logits.requires_grad:
         return _TopkDistill.apply(logits, ids, top, float(temperature), row_weight, factor, reduced)
-    call = _Distill(logits, ids, top, float(temperature), row_weight, factor)
-    total = torch.empty((), device=logits.device, dtype=torch.float32) if reduced else None
-    losses = call.forward(torch.empty((rows, 2), device=logits.device, dtype=torch.float32), total, None)
+    losses, total, _, _ = _distill(logits, ids, top, float(temperature), row_weight, factor, reduced, False)
     return total if reduced else losses
 
 

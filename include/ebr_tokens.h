@@ -28,7 +28,8 @@ int ebr_scaled_embedding(int w_dtype, int out_dtype, int id_type, int64_t n, int
                          const void* ids, const void* w, int64_t w_stride, void* out, void* stream);
 
 /* Its gradient with respect to the table: dW[v, :] = round(scale * sum over t with ids[t] = v of g[t, :]), g [n, C] of
- * type g_dtype (row stride g_stride, unit column stride), dW [V, C] of type w_dtype, contiguous, every element written.
+ * type g_dtype (row stride g_stride, unit column stride), dW [V, C] of type w_dtype, contiguous,
+ * 16-byte aligned, every element written.
  * The sum runs over the tokens sorted by id. Ids outside [0, V) contribute nothing. n < 2^30, V < 2^30. */
 int ebr_scaled_embedding_grad(int g_dtype, int w_dtype, int id_type, int64_t n, int64_t V, int64_t C, double scale,
                               const void* ids, const void* g, int64_t g_stride, void* dw, void* scratch,
