@@ -274,7 +274,7 @@ int check_embedding(int id_type, int64_t n, int64_t V, int64_t C, int64_t stride
 int64_t grad_chunk_rows(int64_t n, int64_t C) {
   const int64_t blocks = (C + 255) / 256;
   int64_t r = 8;
-  while (r < 256 && n * blocks / r > 3000) r *= 2;
+  while (r < 256 && n * blocks / r > 3500) r *= 2;
   return r;
 }
 
