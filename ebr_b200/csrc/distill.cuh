@@ -437,19 +437,23 @@ __device__ __forceinline__ void zero_granules(const Granules<T>& r, int lo, int 
   }
 }
 
-// weights[n] = the row's weight, 0 where it has no entry: what the dense kernel has to know of the teacher, found before it,
-// because there the dependent reads would stand in every row's way.
-__global__ void __launch_bounds__(256) distill_weights_kernel(const __grid_constant__ Args a, float* weights) {
-  const int64_t n = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (n >= a.N) return;
+// Row n's weight, 0 where it has no entry: what the dense kernel has to know of the teacher. By a whole warp.
+__device__ __forceinline__ float weight_by_warp(const Args& a, int64_t n) {
   bool any = false;
   for (int k = threadIdx.x & 31; k < a.K; k += 32) {
     const int i = top_id(a, n * a.K + k);
     const float t = top_value(a, n * a.K + k);
     any |= i >= 0 && t != -INFINITY;
   }
-  any = __any_sync(0xffffffffu, any);
-  if ((threadIdx.x & 31) == 0) weights[n] = !any ? 0.f : a.row_weight ? a.row_weight[n] : 1.f;
+  return !__any_sync(0xffffffffu, any) ? 0.f : a.row_weight ? a.row_weight[n] : 1.f;
+}
+
+// The same for all rows, before the dense kernel, because there the dependent reads would stand in every row's way.
+__global__ void __launch_bounds__(256) distill_weights_kernel(const __grid_constant__ Args a, float* weights) {
+  const int64_t n = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  if (n >= a.N) return;
+  const float w = weight_by_warp(a, n);
+  if ((threadIdx.x & 31) == 0) weights[n] = w;
 }
 
 // The dense part of long rows: the statistics, and grad = c_n q where a.grad is set, so that the logits cross HBM once.
@@ -509,12 +513,15 @@ __global__ void __launch_bounds__(kWarps * 32 + 32) distill_row_kernel(const __g
     cluster_wait();  // every CTA's barriers are there before another one arrives at them
   }
   const int first = static_cast<int>(blockIdx.x) / slices;
+  // weights is NULL where no cluster has a second row: the warps then read the row's entries themselves
+  const float own = weights ? 0.f : weight_by_warp(a, first);
+  auto weight_of = [&](int n) { return weights ? weights[n] : own; };
   if (warp == kWarps) {
     if (lane == 0) {
       const uint64_t once = policy_once(), again = policy_again();
       int slot = 0, round = 0;
       for (int n = first; n < rows; n += step) {
-        if (weights[n] == 0.f) continue;
+        if (weight_of(n) == 0.f) continue;
         const Slice s = slice_of(row_of(n));
         const int loads = s.chunks + (a.grad ? s.chunks - s.kept : 0);
         for (int j = 0; j < loads; ++j) {
@@ -534,10 +541,10 @@ __global__ void __launch_bounds__(kWarps * 32 + 32) distill_row_kernel(const __g
     auto advance = [&] {
       if (++slot == slots) slot = 0, ++round;
     };
-    float weight = first < rows ? weights[first] : 0.f;
+    float weight = first < rows ? weight_of(first) : 0.f;
     for (int n = first; n < rows; n += step) {
       const float now = weight;
-      weight = n + step < rows ? weights[n + step] : 0.f;
+      weight = n + step < rows ? weight_of(n + step) : 0.f;
       T* grad = a.grad ? static_cast<T*>(a.grad) + n * a.grad_stride : nullptr;
       if (now == 0.f) {  // the same in every warp of the cluster
         if (grad) {

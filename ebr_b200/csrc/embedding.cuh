@@ -345,5 +345,43 @@ __global__ void __launch_bounds__(kJoinWarps * 32) grad_join_kernel(int n, int r
   }
 }
 
+// Few tokens: a warp owns a table row's part and goes through all ids itself, adding the rows of its own in their order. No
+// sort, no zeroing, no joining: one launch, where the launches are the cost.
+template <typename TG, typename TW, int V>
+__global__ void __launch_bounds__(kGradWarps * 32) grad_few_kernel(IdSource src, int n, int64_t C,
+                                                                   const TG* __restrict__ g, int64_t g_stride,
+                                                                   float scale, TW* __restrict__ dw) {
+  constexpr int kAhead = 8;
+  const int lane = threadIdx.x & 31;
+  const int64_t v = static_cast<int64_t>(blockIdx.x) * kGradWarps + (threadIdx.x >> 5);
+  if (v >= src.range) return;
+  const int64_t c = (static_cast<int64_t>(blockIdx.y) * 32 + lane) * V;
+  float acc[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) acc[i] = 0.f;
+  for (int t0 = 0; t0 < n; t0 += 32) {
+    unsigned mine = __ballot_sync(0xffffffffu, t0 + lane < n && src.key(t0 + lane) == v);
+    while (mine) {
+      Raw<TG, V> r[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (mine && c < C) r[u].load(g + (t0 + __ffs(mine) - 1) * g_stride + c);
+        mine &= mine - 1;
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        float x[V];
+        r[u].widen(x);
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] += x[i];
+      }
+    }
+  }
+  if (c >= C) return;
+#pragma unroll
+  for (int i = 0; i < V; ++i) acc[i] *= scale;
+  store_f<TW, V>(dw + v * C + c, acc);
+}
+
 }  // namespace embed
 }  // namespace ebr

@@ -6,7 +6,8 @@
 //
 // All are bound by HBM. A warp serves one token, so that x[t] is read once for its K rows and y[t] is written once, and
 // every access is a whole vector per lane of one row. kU vectors of a row, and those of several rows in the combine, are
-// in flight at once. The rows' numbers and weights of up to 32 slots sit in the lanes. Rows of no slot are zeroed by
+// in flight at once; where the tokens are few, several warps
+// (blockIdx.y) share a token's columns. The rows' numbers and weights of up to 32 slots sit in the lanes. Rows of no slot are zeroed by
 // further blocks of the same launch.
 #pragma once
 
@@ -40,6 +41,7 @@ __global__ void __launch_bounds__(kWarps * 32) scatter_kernel(int64_t T_, int K,
                                                               TW* __restrict__ dots, int token_blocks) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (static_cast<int>(blockIdx.x) >= token_blocks) {
+    if (blockIdx.y > 0) return;
     const int64_t r0 = static_cast<int64_t>(blockIdx.x - token_blocks) * kZeroRows;
     for (int64_t r = r0 + warp; r < min(rows, r0 + kZeroRows); r += kWarps) {
       if (slot_of[r] >= 0) continue;
@@ -49,6 +51,7 @@ __global__ void __launch_bounds__(kWarps * 32) scatter_kernel(int64_t T_, int K,
     return;
   }
   const int64_t step = static_cast<int64_t>(token_blocks) * kWarps;
+  const int64_t first = static_cast<int64_t>(blockIdx.y) * kU * 32 * V, stride = static_cast<int64_t>(gridDim.y) * kU * 32 * V;
   int64_t t = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
   int my_row = -1, next_row;
   float my_w = 1.f, next_w;
@@ -60,7 +63,7 @@ __global__ void __launch_bounds__(kWarps * 32) scatter_kernel(int64_t T_, int K,
     float my_dot = 0.f;
     if (k0 > 0) slots_of(row_of, weights, t, K, k0, lane, &my_row, &my_w);
     const int slots = min(32, K - k0);
-    for (int64_t c0 = lane * V; c0 < C + lane * V; c0 += kU * 32 * V) {  // the same trips for all lanes
+    for (int64_t c0 = first + lane * V; c0 < C + lane * V; c0 += stride) {  // the same trips for all lanes
       Raw<T, V> a[kU];
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
@@ -123,13 +126,14 @@ __global__ void __launch_bounds__(kWarps * 32) combine_kernel(int64_t T_, int K,
   constexpr int kRows = 2;  // rows in flight
   const int lane = threadIdx.x & 31;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps;
+  const int64_t first = static_cast<int64_t>(blockIdx.y) * kU * 32 * V, stride = static_cast<int64_t>(gridDim.y) * kU * 32 * V;
   int64_t t = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
   int my_row = -1, next_row;
   float my_w = 1.f, next_w;
   if (t < T_) slots_of(row_of, weights, t, K, 0, lane, &my_row, &my_w);
   for (; t < T_; t += step, my_row = next_row, my_w = next_w) {
   if (t + step < T_) slots_of(row_of, weights, t + step, K, 0, lane, &next_row, &next_w);
-  for (int64_t c0 = lane * V; c0 < C + lane * V; c0 += kU * 32 * V) {  // the same trips for all lanes
+  for (int64_t c0 = first + lane * V; c0 < C + lane * V; c0 += stride) {  // the same trips for all lanes
     float acc[kU][V];
 #pragma unroll
     for (int u = 0; u < kU; ++u)

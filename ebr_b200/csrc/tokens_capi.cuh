@@ -79,7 +79,7 @@ int with_width(int v, Fn&& fn) {
 // ------------------------------------------------------------------------------------------------ sort
 
 // Keys that one cluster of 16 CTAs ranks in registers, and those up to which it is used even where nothing runs beside
-// it: 18,006 slots take 8.7 us in a cluster; 124,416 take 15.6 there and XX in two kernels over the whole GPU.
+// it: 18,006 slots take 8.7 us in a cluster; 124,416 take 15.6 there and 7.0 in two kernels over the whole GPU.
 constexpr int64_t kClusterKeys = 16 * int64_t{ebr::keysort::kSortThreads} * 16;
 constexpr int64_t kClusterAlone = 32 * 1024;
 
@@ -278,6 +278,10 @@ int64_t grad_chunk_rows(int64_t n, int64_t C) {
   return r;
 }
 
+// Gradients that one launch makes, each warp looking through all ids: up to 128 tokens (81 board tokens: 3.5 us, 12.1 by way of
+// the sort; the worst of 256, all of one id, would be 23 against 13) and as many warps as some waves of them.
+bool grad_by_few(int64_t n, int64_t V, int64_t C) { return n <= 128 && V * ((C + 255) / 256) <= 65536; }
+
 // ------------------------------------------------------------------------------------------------ distillation
 
 constexpr int64_t kMaxVocabulary = int64_t{1} << 19;
@@ -326,6 +330,14 @@ int launch_distill_row(int device, const ebr::distill::Args& a, int slices, int 
   cfg.blockDim = dim3(kWarps * 32 + 32);
   cfg.dynamicSmemBytes = static_cast<size_t>(slots) * kWarps * kU * 512;
   const int64_t clusters = std::max<int64_t>(1, std::min<int64_t>(a.N, per_sm * sm_count(device) / slices));
+  // The rows' weights come from a kernel of their own (in `losses`, which the last kernel writes), unless no cluster has a
+  // second row: 12 rows of 151,665 float16 logits take 8.2 us without it, 9.5 with it.
+  const float* weights = clusters < a.N ? a.losses : nullptr;
+  if (weights) {
+    ebr::distill::distill_weights_kernel<<<static_cast<unsigned>((a.N + 7) / 8), 256, 0, st>>>(a, a.losses);
+    const int rc = check_launch("topk_distill weights");
+    if (rc != EBR_OK) return rc;
+  }
   cfg.gridDim = dim3(static_cast<unsigned>(clusters * slices));
   cfg.stream = st;
   cudaLaunchAttribute at[1];
@@ -333,7 +345,7 @@ int launch_distill_row(int device, const ebr::distill::Args& a, int slices, int 
   at[0].val.clusterDim = {static_cast<unsigned>(slices), 1, 1};
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, static_cast<const float*>(a.losses), slices, granules, slots);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, weights, slices, granules, slots);
   if (e != cudaSuccess) return cuda_error(e, "topk_distill");
   return check_launch("topk_distill");
 }
@@ -362,15 +374,11 @@ int launch_distill(int device, const ebr::distill::Args& a, cudaStream_t st) {
   while (slices < ebr::distill::kMaxSlices && a.N * slices < 2 * sm_count(device) && (total + slices - 1) / slices > 256)
     slices *= 2;
   const int granules = static_cast<int>((total + slices - 1) / slices);
-  // the rows' weights travel in `losses`, which the last kernel writes
-  ebr::distill::distill_weights_kernel<<<static_cast<unsigned>((a.N + 7) / 8), 256, 0, st>>>(a, a.losses);
-  int rc = check_launch("topk_distill weights");
-  if (rc != EBR_OK) return rc;
   // Rows above 128 KB: rings of six 16 KB chunks, two on an SM, keep more of the row between the passes; shorter rows want
   // more rows in flight: rings of four 8 KB chunks, six on an SM. bfloat16 at 2.1 GB: V = 131,072 takes 0.45 ms with the
   // first, 0.53 with the second; V = 32,768 takes 0.56 and 0.50.
-  rc = granules > 8192 ? launch_distill_row<T, 8, 4>(device, a, slices, granules, 6, 2, st)
-                       : launch_distill_row<T, 4, 4>(device, a, slices, granules, 4, 6, st);
+  const int rc = granules > 8192 ? launch_distill_row<T, 8, 4>(device, a, slices, granules, 6, 2, st)
+                                 : launch_distill_row<T, 4, 4>(device, a, slices, granules, 4, 6, st);
   return rc != EBR_OK ? rc : launch_distill_entries<T, true>(a, st);
 }
 
@@ -465,6 +473,7 @@ int ebr_scaled_embedding(int w_dtype, int out_dtype, int id_type, int64_t n, int
 
 size_t ebr_scaled_embedding_grad_scratch_bytes(int64_t n, int64_t V, int64_t C) {
   if (n <= 0 || V < 1 || C < 1 || n >= kMaxSortKeys || V >= kMaxSortKeys || C > (1 << 24)) return 0;
+  if (grad_by_few(n, V, C)) return 0;
   const int passes = digit_passes(V);
   const int64_t chunks = (n + grad_chunk_rows(n, C) - 1) / grad_chunk_rows(n, C);
   return sort_scratch(n, int64_t{1} << digit_bits(V, passes), passes, false) +
@@ -489,9 +498,28 @@ int ebr_scaled_embedding_grad(int g_dtype, int w_dtype, int id_type, int64_t n, 
   }
   if (!ids || !g) return set_error(EBR_ERR_NULL, "scaled_embedding_grad: NULL pointer%s%s");
   if (!aligned16(dw)) return set_error(EBR_ERR_STRIDE, "scaled_embedding_grad: dW must be 16-byte aligned%s%s");
-  if (!scratch || !aligned16(scratch) || scratch_bytes < ebr_scaled_embedding_grad_scratch_bytes(n, V, C))
+  const size_t need = ebr_scaled_embedding_grad_scratch_bytes(n, V, C);
+  if (need && (!scratch || !aligned16(scratch) || scratch_bytes < need))
     return set_error(EBR_ERR_SCRATCH, "scaled_embedding_grad: scratch too small or unaligned%s%s");
   if ((rc = check_device(&device)) != EBR_OK) return rc;
+  if (!need)
+    return with_types(g_dtype, w_dtype, [&](auto* gt, auto* wt) -> int {
+      using TG = std::remove_pointer_t<decltype(gt)>;
+      using TW = std::remove_pointer_t<decltype(wt)>;
+      using namespace ebr::embed;
+      constexpr int kMost = static_cast<int>(16 / sizeof(TG));
+      const int v = access_width(kMost, C, {{g, g_stride, int(sizeof(TG))}, {dw, C, int(sizeof(TW))}});
+      return with_width<kMost>(v, [&](auto vc) -> int {
+        constexpr int V_ = decltype(vc)::value;
+        const int64_t cols = (C + 32 * V_ - 1) / (32 * V_);
+        if (cols > 65535) return set_error(EBR_ERR_SHAPE, "scaled_embedding_grad: row too long%s%s");
+        grad_few_kernel<TG, TW, V_><<<dim3(static_cast<unsigned>((V + kGradWarps - 1) / kGradWarps),
+                                           static_cast<unsigned>(cols)), kGradWarps * 32, 0, st>>>(
+            IdSource{ids, id_type == EBR_INT64, static_cast<int>(V)}, static_cast<int>(n), C, static_cast<const TG*>(g),
+            g_stride, static_cast<float>(scale), static_cast<TW*>(dw));
+        return check_launch("scaled_embedding_grad");
+      });
+    });
   const int passes = digit_passes(V), bits = digit_bits(V, passes);
   int *key = nullptr, *order = nullptr;
   const IdSource src{ids, id_type == EBR_INT64, static_cast<int>(V)};
@@ -531,8 +559,14 @@ int ebr_scaled_embedding_grad(int g_dtype, int w_dtype, int id_type, int64_t n, 
 }  // extern "C"
 
 namespace {
-int64_t expert_blocks(int device, int64_t T) {
-  return std::min<int64_t>((T + ebr::experts::kWarps - 1) / ebr::experts::kWarps, 16 * int64_t{sm_count(device)});
+// Blocks along the tokens, each warp walking over several of them where there are many (board batch: dispatch 42 us with a
+// warp for each token, 38 so), and along the columns, where the tokens alone leave less than 96 warps to an SM (3,001
+// tokens of 999 float32, six rows each: cold, combine 54 us without, 29 with).
+dim3 expert_grid(int device, int64_t T, int64_t C, int per_trip, bool split) {
+  const int64_t warps = int64_t{96} * sm_count(device);
+  const int64_t parts = split ? std::max<int64_t>(1, std::min((C + per_trip - 1) / per_trip, warps / std::max<int64_t>(T, 1))) : 1;
+  const int64_t blocks = std::min<int64_t>((T + ebr::experts::kWarps - 1) / ebr::experts::kWarps, 16 * int64_t{sm_count(device)});
+  return dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(std::min<int64_t>(parts, 64)));
 }
 }  // namespace
 
@@ -603,9 +637,10 @@ int ebr_expert_scatter(int dtype, int weight_dtype, int64_t T, int64_t K, int64_
         auto launch = [&](auto* wtag, auto with_dots) -> int {
           using TW = std::remove_pointer_t<decltype(wtag)>;
           using namespace ebr::experts;
-          const int64_t tb = expert_blocks(device, T);
+          const dim3 grid = expert_grid(device, T, C, unroll_of(V_) * 32 * V_, dots == nullptr);
+          const int64_t tb = grid.x;
           const int64_t zb = rows_out ? (rows + kZeroRows - 1) / kZeroRows : 0;
-          scatter_kernel<T_, TW, V_, unroll_of(V_), decltype(with_dots)::value><<<static_cast<unsigned>(tb + zb), kWarps * 32, 0, st>>>(
+          scatter_kernel<T_, TW, V_, unroll_of(V_), decltype(with_dots)::value><<<dim3(static_cast<unsigned>(tb + zb), grid.y), kWarps * 32, 0, st>>>(
               T, static_cast<int>(K), C, rows, static_cast<const T_*>(x), x_stride, row_of, slot_of,
               static_cast<const TW*>(weights), static_cast<const T_*>(rows_in), static_cast<T_*>(rows_out),
               static_cast<TW*>(dots), static_cast<int>(tb));
@@ -647,7 +682,7 @@ int ebr_expert_combine(int dtype, int weight_dtype, int64_t T, int64_t K, int64_
         auto launch = [&](auto* wtag) -> int {
           using TW = std::remove_pointer_t<decltype(wtag)>;
           using namespace ebr::experts;
-          combine_kernel<T_, TW, V_, unroll_of(V_)><<<static_cast<unsigned>(expert_blocks(device, T)), kWarps * 32, 0, st>>>(
+          combine_kernel<T_, TW, V_, unroll_of(V_)><<<expert_grid(device, T, C, unroll_of(V_) * 32 * V_, true), kWarps * 32, 0, st>>>(
               T, static_cast<int>(K), C, static_cast<const T_*>(rows_in), rows_stride, row_of,
               static_cast<const TW*>(weights), static_cast<T_*>(y));
           return check_launch("expert_combine");

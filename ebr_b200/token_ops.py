@@ -75,6 +75,10 @@ def _ptr(t: Optional[Tensor]):
     return None if t is None else t.data_ptr()
 
 
+def _as(t: Tensor, dtype: torch.dtype) -> Tensor:
+    return t if t.dtype == dtype else t.to(dtype)
+
+
 # ---------------------------------------------------------------------------------------------------- embedding
 
 
@@ -144,7 +148,7 @@ def scaled_embedding(tokens: Tensor, weight: Tensor, scale: float = 1.0, dtype: 
     dtype = weight.dtype if dtype is None else dtype
     if dtype not in _DTYPES:
         raise TypeError(f"scaled_embedding: unsupported output dtype {dtype}")
-    tokens = tokens.contiguous()
+    tokens = tokens if tokens.is_contiguous() else tokens.contiguous()
     if torch.is_grad_enabled() and weight.requires_grad:
         return _Embed.apply(weight, tokens, float(scale), dtype)
     return _lookup(tokens, weight, float(scale), dtype)
@@ -207,35 +211,36 @@ def _weight_args(weights: Optional[Tensor], x: Tensor):
         return None, _native.FLOAT32
     if weights.dtype != torch.float32 and weights.dtype != x.dtype:
         weights = weights.float()
-    return weights.contiguous(), _DTYPES[weights.dtype]
+    return weights if weights.is_contiguous() else weights.contiguous(), _DTYPES[weights.dtype]
 
 
 def _scatter(x: Tensor, route: ExpertRoute, weights: Optional[Tensor], rows_in: Optional[Tensor], want_rows: bool,
              dots_dtype: Optional[torch.dtype] = None) -> Tuple[Optional[Tensor], Optional[Tensor]]:  # fmt: skip
     x, stride = _row_view(x)
-    c = x.shape[-1]
+    c, row_of, slot_of = x.shape[-1], route.row_of, route.slot_of
+    k, rows = row_of.shape[-1], slot_of.shape[0]
     weights, code = _weight_args(weights, x)
     if weights is None and dots_dtype is not None:
         code = _DTYPES[dots_dtype]
-    out = x.new_empty((route.rows, c)) if want_rows else None
+    out = x.new_empty((rows, c)) if want_rows else None
     dots = None
     if rows_in is not None:
-        rows_in = rows_in.to(x.dtype).contiguous()
-        dots = x.new_empty(route.row_of.shape, dtype=torch.float32 if code == _native.FLOAT32 else x.dtype)
-    _call("expert_scatter", x.device, _native.lib().ebr_expert_scatter, _DTYPES[x.dtype], code,
-          route.row_of.numel() // route.top_k, route.top_k, c, route.rows, x.data_ptr(), stride, route.row_of.data_ptr(),
-          route.slot_of.data_ptr(), _ptr(weights), _ptr(rows_in), _ptr(out), _ptr(dots))  # fmt: skip
+        rows_in = _as(rows_in, x.dtype).contiguous()
+        dots = x.new_empty(row_of.shape, dtype=torch.float32 if code == _native.FLOAT32 else x.dtype)
+    _call("expert_scatter", x.device, _native.lib().ebr_expert_scatter, _DTYPES[x.dtype], code, row_of.numel() // k, k, c,
+          rows, x.data_ptr(), stride, row_of.data_ptr(), slot_of.data_ptr(), _ptr(weights), _ptr(rows_in), _ptr(out),
+          _ptr(dots))  # fmt: skip
     return out, dots
 
 
 def _combine(rows: Tensor, route: ExpertRoute, weights: Optional[Tensor]) -> Tensor:
     rows, stride = _row_view(rows)
-    c = rows.shape[-1]
+    c, row_of = rows.shape[-1], route.row_of
+    k = row_of.shape[-1]
     weights, code = _weight_args(weights, rows)
-    y = rows.new_empty((*route.row_of.shape[:-1], c))
-    _call("expert_combine", rows.device, _native.lib().ebr_expert_combine, _DTYPES[rows.dtype], code,
-          route.row_of.numel() // route.top_k, route.top_k, c, rows.data_ptr(), stride, route.row_of.data_ptr(),
-          _ptr(weights), y.data_ptr())  # fmt: skip
+    y = rows.new_empty((*row_of.shape[:-1], c))
+    _call("expert_combine", rows.device, _native.lib().ebr_expert_combine, _DTYPES[rows.dtype], code, row_of.numel() // k,
+          k, c, rows.data_ptr(), stride, row_of.data_ptr(), _ptr(weights), y.data_ptr())  # fmt: skip
     return y
 
 
@@ -246,12 +251,15 @@ class _Dispatch(torch.autograd.Function):
     def forward(ctx, x: Tensor, weights: Optional[Tensor], route: ExpertRoute) -> Tensor:
         ctx.route = route
         ctx.weighted = weights is not None
-        ctx.save_for_backward(*((x, weights) if ctx.weighted else ()))
+        if ctx.weighted:
+            ctx.save_for_backward(x, weights)
         return _scatter(x, route, weights, None, True)[0]
 
     @staticmethod
     def backward(ctx, g: Tensor):
         route = ctx.route
+        if not ctx.weighted and not torch.is_grad_enabled():
+            return _combine(g, route, None), None, None
         x, weights = ctx.saved_tensors if ctx.weighted else (None, None)
         gx = _Combine.apply(g, weights, route) if ctx.needs_input_grad[0] else None
         gw = _RowDots.apply(x, g, route, weights.dtype) if ctx.weighted and ctx.needs_input_grad[1] else None
@@ -265,7 +273,8 @@ class _Combine(torch.autograd.Function):
     def forward(ctx, rows: Tensor, weights: Optional[Tensor], route: ExpertRoute) -> Tensor:
         ctx.route = route
         ctx.weighted = weights is not None
-        ctx.save_for_backward(*((rows, weights) if ctx.weighted else ()))
+        if ctx.weighted:
+            ctx.save_for_backward(rows, weights)
         return _combine(rows, route, weights)
 
     @staticmethod
@@ -274,8 +283,8 @@ class _Combine(torch.autograd.Function):
         rows, weights = ctx.saved_tensors if ctx.weighted else (None, None)
         need_rows, need_weights = ctx.needs_input_grad[:2]
         if need_rows and need_weights and ctx.weighted and not torch.is_grad_enabled():
-            grows, gw = _scatter(g.to(rows.dtype), route, weights, rows, True)  # both in one pass over g and the rows
-            return grows, gw.to(weights.dtype), None
+            grows, gw = _scatter(_as(g, rows.dtype), route, weights, rows, True)  # both in one pass over g and the rows
+            return grows, _as(gw, weights.dtype), None
         grows = _Dispatch.apply(g, weights, route) if need_rows else None
         gw = _RowDots.apply(g, rows, route, weights.dtype) if ctx.weighted and need_weights else None
         return grows, gw, None
