@@ -312,6 +312,11 @@ struct Granules {
   __device__ __forceinline__ int first_whole() const { return phase ? 1 : 0; }
   __device__ __forceinline__ int end_whole() const { return (phase + V) / kE; }
   __device__ __forceinline__ int first(int g) const { return g * kE - phase; }  // element
+  // The ragged granule at the front (end 0) or at the back (end 1), -1 where there is none or another `end`.
+  __device__ __forceinline__ int ragged_end(int end) const {
+    const int g = end == 0 ? 0 : end == 1 ? count() - 1 : -1;
+    return g >= end && !whole(g) ? g : -1;
+  }
 };
 
 // mult * 2^((v - m) * scale) for a granule.
@@ -557,12 +562,8 @@ __global__ void __launch_bounds__(kWarps * 32 + 32) distill_row_kernel(const __g
       }
       const Granules<T> row = row_of(n);
       const Slice s = slice_of(row);
-      int end = -1;  // this thread's ragged granule
-      if (threadIdx.x < 2) {
-        const int g = threadIdx.x == 0 ? 0 : row.count() - 1;
-        if (g >= slice * slice_granules && g < (slice + 1) * slice_granules && !row.whole(g) && (threadIdx.x == 0 || g > 0))
-          end = g;
-      }
+      int end = row.ragged_end(static_cast<int>(threadIdx.x));  // this thread's ragged granule
+      if (end < slice * slice_granules || end >= (slice + 1) * slice_granules) end = -1;
       const uint4 ragged_end = end >= 0 ? ragged(row, end) : Granule<T>::none();
       // first pass: the statistics, the maximum the warp's own
       Stat st;
@@ -575,7 +576,11 @@ __global__ void __launch_bounds__(kWarps * 32 + 32) distill_row_kernel(const __g
         const int left = s.count - c * kChunk - part;
         uint4 v[kU];
 #pragma unroll
-        for (int u = 0; u < kU; ++u) v[u] = u * 32 < left ? chunk[u * 32] : Granule<T>::none();
+        for (int u = 0; u < kU; ++u) v[u] = chunk[u * 32];  // in the ring, if not of this row
+        if (c + 1 == s.chunks)
+#pragma unroll
+          for (int u = 0; u < kU; ++u)
+            if (u * 32 >= left) v[u] = Granule<T>::none();
         uint4 most = v[0];
 #pragma unroll
         for (int u = 1; u < kU; ++u) most = Granule<T>::larger(most, v[u]);
@@ -644,7 +649,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32) distill_row_kernel(const __g
         const int left = s.count - c * kChunk - part, from = s.begin + (c * kChunk + part) * kE;
         uint4 v[kU];
 #pragma unroll
-        for (int u = 0; u < kU; ++u) v[u] = u * 32 < left ? chunk[u * 32] : Granule<T>::none();
+        for (int u = 0; u < kU; ++u) v[u] = chunk[u * 32];
 #pragma unroll
         for (int u = 0; u < kU; ++u) {
           v[u] = grad_granule<T>(v[u], all.m, a.exp2_scale, mult);
@@ -870,29 +875,40 @@ __global__ void __launch_bounds__(kMidWarps * 32) distill_warp_kernel(const __gr
     return;
   }
   const Granules<T> row(static_cast<const T*>(a.logits) + n * a.logits_stride, a.V);
-  const int count = row.count();
-  auto load = [&](int g) {
-    if (g >= count) return Granule<T>::none();
-    return row.whole(g) ? *reinterpret_cast<const uint4*>(row.row + row.first(g)) : ragged(row, g);
-  };
+  // The whole granules [begin, end) go by vectors; the row's ragged ends, at most two, belong to lanes 0 and 1. A lane past
+  // the last whole granule reads that one again and drops it: no branch stands between the loads.
+  const int begin = row.first_whole(), end = row.end_whole();
+  const int edge = row.ragged_end(lane);
+  const uint4 ragged_end = edge >= 0 ? ragged(row, edge) : Granule<T>::none();
+  auto load = [&](int g) { return *reinterpret_cast<const uint4*>(row.row + row.first(min(g, end - 1))); };
   float m, sum;
   if constexpr (kStats) {
     Stat st;
-    for (int g0 = lane; g0 < count + lane; g0 += kU * 32) {  // the same trips for all lanes
-      uint4 v[kU];
-#pragma unroll
-      for (int u = 0; u < kU; ++u) v[u] = load(g0 + u * 32);
-      uint4 most = v[0];
-#pragma unroll
-      for (int u = 1; u < kU; ++u) most = Granule<T>::larger(most, v[u]);
+    auto add = [&](const uint4& most, auto&& terms) {
       const float top = warp_largest(Granule<T>::largest(most));
       if (top > st.m) {
         st.s *= exp2_approx((st.m - top) * a.exp2_scale);
         st.m = top;
       }
-      const float base = st.base();
+      st.s += terms(st.base());
+    };
+    add(ragged_end, [&](float base) { return exp2_sum<T>(ragged_end, base, a.exp2_scale); });
+    for (int g0 = begin + lane; g0 < end + lane; g0 += kU * 32) {  // the same trips for all lanes
+      uint4 v[kU];
 #pragma unroll
-      for (int u = 0; u < kU; ++u) st.s += exp2_sum<T>(v[u], base, a.exp2_scale);
+      for (int u = 0; u < kU; ++u) v[u] = load(g0 + u * 32);
+#pragma unroll
+      for (int u = 0; u < kU; ++u)
+        if (g0 + u * 32 >= end) v[u] = Granule<T>::none();
+      uint4 most = v[0];
+#pragma unroll
+      for (int u = 1; u < kU; ++u) most = Granule<T>::larger(most, v[u]);
+      add(most, [&](float base) {
+        float t = 0.f;
+#pragma unroll
+        for (int u = 0; u < kU; ++u) t += exp2_sum<T>(v[u], base, a.exp2_scale);
+        return t;
+      });
     }
     m = st.m;
     sum = lanes_sum<32>(st.s);
@@ -909,21 +925,24 @@ __global__ void __launch_bounds__(kMidWarps * 32) distill_warp_kernel(const __gr
   const float up = a.upstream ? a.upstream[n * a.upstream_stride] : 1.f;
   const float coef = a.factor * up * weight * a.tau, inv_sum = 1.f / sum, mult = coef * inv_sum;
   const bool same = ((reinterpret_cast<uintptr_t>(grad) ^ reinterpret_cast<uintptr_t>(row.row)) & 15) == 0;
-  for (int g0 = lane; g0 < count; g0 += kU * 32) {
+  if (edge >= 0)
+    store_elements<T>(grad_granule<T>(ragged_end, m, a.exp2_scale, mult), row.first(edge), row.V, grad);
+  for (int g0 = begin + lane; g0 < end + lane; g0 += kU * 32) {
     uint4 v[kU];
 #pragma unroll
     for (int u = 0; u < kU; ++u) v[u] = load(g0 + u * 32);
 #pragma unroll
     for (int u = 0; u < kU; ++u) {
       const int g = g0 + u * 32;
-      if (g >= count) continue;
       v[u] = grad_granule<T>(v[u], m, a.exp2_scale, mult);
-      if (same && row.whole(g))
+      if (g >= end) continue;
+      if (same)
         *reinterpret_cast<uint4*>(grad + row.first(g)) = v[u];
       else
         store_elements<T>(v[u], row.first(g), row.V, grad);
     }
   }
+  __syncwarp();  // the dense pass is complete
   e.store<T>(a, row.row, m, inv_sum, coef, grad);
 }
 

@@ -132,18 +132,15 @@ __global__ void __launch_bounds__(kLookupWarps * 32) lookup_kernel(IdSource src,
   TO* dst = out + t0 * C + c0;
   for (int j0 = 0; j0 < tokens; j0 += kRows) {
     float v[kRows][kU][V];
+    int id[kRows];
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
-      const int id = __shfl_sync(0xffffffffu, my_id, (j0 + r) & 31);
+      // Lanes past the row and ids of no row read somewhere valid: no branch stands between the loads.
+      id[r] = __shfl_sync(0xffffffffu, my_id, (j0 + r) & 31);
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
         const int64_t c = c0 + u * 32 * V;
-        if (id < src.range && c < C && j0 + r < tokens) {
-          load_f<TW, V>(w + id * w_stride + c, v[r][u]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < V; ++i) v[r][u][i] = 0.f;
-        }
+        load_f<TW, V>(w + (id[r] < src.range ? id[r] : 0) * w_stride + (c < C ? c : 0), v[r][u]);
       }
     }
 #pragma unroll
@@ -152,7 +149,7 @@ __global__ void __launch_bounds__(kLookupWarps * 32) lookup_kernel(IdSource src,
       for (int u = 0; u < kU; ++u) {
         if (j0 + r >= tokens || c0 + u * 32 * V >= C) continue;
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[r][u][i] *= scale;
+        for (int i = 0; i < V; ++i) v[r][u][i] = id[r] < src.range ? v[r][u][i] * scale : 0.f;
         store_f<TO, V>(dst + (j0 + r) * C + u * 32 * V, v[r][u]);
       }
   }
@@ -214,11 +211,12 @@ __global__ void __launch_bounds__(kGradWarps * 32) grad_chunk_kernel(int n, int 
       Raw<TG, V> v[kAhead];
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
+        // Lanes past the row and rows past the last read somewhere valid: no branch stands between the loads.
         const int64_t row = __shfl_sync(0xffffffffu, my_row, (j0 + u) & 31);
-        if (j0 + u < valid && live) v[u].load(g + row * g_stride + c);
+        v[u].load(g + row * g_stride + (live ? c : 0));
       }
       const int last = __shfl_sync(0xffffffffu, my_key, min(j0 + kAhead, valid) - 1);
-      if (last == cur) {  // one run: the rows past `valid` add zeros
+      if (last == cur && j0 + kAhead <= valid) {  // one run
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) add(v[u]);
       } else {

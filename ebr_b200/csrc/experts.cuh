@@ -153,8 +153,9 @@ __global__ void __launch_bounds__(kWarps * 32) combine_kernel(int64_t T_, int K,
           if (k + r >= slots) row[r] = -1;
 #pragma unroll
           for (int u = 0; u < kU; ++u) {
+            // Lanes past the row and dropped slots read somewhere valid: no branch stands between the loads.
             const int64_t c = c0 + u * 32 * V;
-            if (row[r] >= 0 && c < C) b[r][u].load(rows_in + row[r] * rows_stride + c);
+            b[r][u].load(rows_in + max(row[r], 0) * rows_stride + (c < C ? c : 0));
           }
         }
 #pragma unroll

@@ -565,7 +565,7 @@ namespace {
 dim3 expert_grid(int device, int64_t T, int64_t C, int per_trip, bool split) {
   const int64_t warps = int64_t{96} * sm_count(device);
   const int64_t parts = split ? std::max<int64_t>(1, std::min((C + per_trip - 1) / per_trip, warps / std::max<int64_t>(T, 1))) : 1;
-  const int64_t blocks = std::min<int64_t>((T + ebr::experts::kWarps - 1) / ebr::experts::kWarps, 16 * int64_t{sm_count(device)});
+  const int64_t blocks = std::min<int64_t>((T + ebr::experts::kWarps - 1) / ebr::experts::kWarps, 24 * int64_t{sm_count(device)});
   return dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(std::min<int64_t>(parts, 64)));
 }
 }  // namespace
