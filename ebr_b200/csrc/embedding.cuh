@@ -343,37 +343,53 @@ __global__ void __launch_bounds__(kJoinWarps * 32) grad_join_kernel(int n, int r
   }
 }
 
-// Few tokens: a warp owns a table row's part and goes through all ids itself, adding the rows of its own in their order. No
-// sort, no zeroing, no joining: one launch, where the launches are the cost.
-template <typename TG, typename TW, int V>
+// Few tokens: kShare warps own a table row's part and go through all ids themselves, each through its stretch of them, adding
+// the rows of their own in their order. No sort, no zeroing, no joining: one launch, where the launches are the cost.
+template <typename TG, typename TW, int V, int kShare>
 __global__ void __launch_bounds__(kGradWarps * 32) grad_few_kernel(IdSource src, int n, int64_t C,
                                                                    const TG* __restrict__ g, int64_t g_stride,
                                                                    float scale, TW* __restrict__ dw) {
-  constexpr int kAhead = 8;
-  const int lane = threadIdx.x & 31;
-  const int64_t v = static_cast<int64_t>(blockIdx.x) * kGradWarps + (threadIdx.x >> 5);
-  if (v >= src.range) return;
+  constexpr int kAhead = 8, kOwners = kGradWarps / kShare;
+  __shared__ float sums[kShare > 1 ? kGradWarps : 1][32][V];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % kShare;
+  const int64_t v = static_cast<int64_t>(blockIdx.x) * kOwners + warp / kShare;
+  if (kShare == 1 && v >= src.range) return;
   const int64_t c = (static_cast<int64_t>(blockIdx.y) * 32 + lane) * V;
+  const int span = ((n + kShare - 1) / kShare + 31) / 32 * 32, end = min(n, (part + 1) * span);
   float acc[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) acc[i] = 0.f;
-  for (int t0 = 0; t0 < n; t0 += 32) {
-    unsigned mine = __ballot_sync(0xffffffffu, t0 + lane < n && src.key(t0 + lane) == v);
+  for (int t0 = part * span; t0 < end; t0 += 32) {
+    unsigned mine = __ballot_sync(0xffffffffu, t0 + lane < end && src.key(t0 + lane) == v);
+    if (v >= src.range) mine = 0;
     while (mine) {
       Raw<TG, V> r[kAhead];
+      unsigned left = mine;
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        if (mine && c < C) r[u].load(g + (t0 + __ffs(mine) - 1) * g_stride + c);
-        mine &= mine - 1;
+      for (int u = 0; u < kAhead; ++u) {  // past the last one: the first again, not used
+        r[u].load(g + (t0 + __ffs(left ? left : mine) - 1) * g_stride + (c < C ? c : 0));
+        left &= left - 1;
       }
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
+        if (!mine) break;
         float x[V];
         r[u].widen(x);
 #pragma unroll
         for (int i = 0; i < V; ++i) acc[i] += x[i];
+        mine &= mine - 1;
       }
     }
+  }
+  if constexpr (kShare > 1) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) sums[warp][lane][i] = acc[i];
+    __syncthreads();
+    if (part > 0 || v >= src.range) return;
+#pragma unroll
+    for (int p = 1; p < kShare; ++p)
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[i] += sums[warp + p][lane][i];
   }
   if (c >= C) return;
 #pragma unroll

@@ -278,9 +278,15 @@ int64_t grad_chunk_rows(int64_t n, int64_t C) {
   return r;
 }
 
-// Gradients that one launch makes, each warp looking through all ids: up to 128 tokens (81 board tokens: 3.5 us, 12.1 by way of
-// the sort; the worst of 256, all of one id, would be 23 against 13) and as many warps as some waves of them.
-bool grad_by_few(int64_t n, int64_t V, int64_t C) { return n <= 128 && V * ((C + 255) / 256) <= 65536; }
+// Gradients that one launch makes, the warps looking through all ids: few tokens, and as many warps as some waves of them. A
+// block owns a table row where the rows are few, up to kSomeTokens (500 tokens over ten ids: 4.2 us, 12.7 by way of the
+// sort), else a warp does, up to kFewTokens.
+constexpr int64_t kFewTokens = 128, kSomeTokens = 512;
+
+bool grad_by_blocks(int64_t n, int64_t V, int64_t C) { return n <= kSomeTokens && V * ((C + 255) / 256) <= 2048; }
+bool grad_by_few(int64_t n, int64_t V, int64_t C) {
+  return grad_by_blocks(n, V, C) || (n <= kFewTokens && V * ((C + 255) / 256) <= 65536);
+}
 
 // ------------------------------------------------------------------------------------------------ distillation
 
@@ -513,10 +519,18 @@ int ebr_scaled_embedding_grad(int g_dtype, int w_dtype, int id_type, int64_t n, 
         constexpr int V_ = decltype(vc)::value;
         const int64_t cols = (C + 32 * V_ - 1) / (32 * V_);
         if (cols > 65535) return set_error(EBR_ERR_SHAPE, "scaled_embedding_grad: row too long%s%s");
-        grad_few_kernel<TG, TW, V_><<<dim3(static_cast<unsigned>((V + kGradWarps - 1) / kGradWarps),
-                                           static_cast<unsigned>(cols)), kGradWarps * 32, 0, st>>>(
-            IdSource{ids, id_type == EBR_INT64, static_cast<int>(V)}, static_cast<int>(n), C, static_cast<const TG*>(g),
-            g_stride, static_cast<float>(scale), static_cast<TW*>(dw));
+        const IdSource src{ids, id_type == EBR_INT64, static_cast<int>(V)};
+        auto launch = [&](auto share) {
+          constexpr int kShare = decltype(share)::value, kOwners = kGradWarps / kShare;
+          grad_few_kernel<TG, TW, V_, kShare><<<dim3(static_cast<unsigned>((V + kOwners - 1) / kOwners),
+                                                     static_cast<unsigned>(cols)), kGradWarps * 32, 0, st>>>(
+              src, static_cast<int>(n), C, static_cast<const TG*>(g), g_stride, static_cast<float>(scale),
+              static_cast<TW*>(dw));
+        };
+        if (grad_by_blocks(n, V, C))
+          launch(std::integral_constant<int, kGradWarps>{});
+        else
+          launch(std::integral_constant<int, 1>{});
         return check_launch("scaled_embedding_grad");
       });
     });

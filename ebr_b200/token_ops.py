@@ -34,6 +34,8 @@ _IDS = {torch.int32: _native.INT32, torch.int64: _native.INT64}
 
 # ---------------------------------------------------------------------------------------------------- plumbing
 
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
 
 def _require(t: Tensor, what: str, name: str, types: dict, device: Optional[torch.device] = None) -> None:
     if not t.is_cuda:
@@ -44,15 +46,19 @@ def _require(t: Tensor, what: str, name: str, types: dict, device: Optional[torc
         raise ValueError(f"{what}: {name} is on {t.device}, the other tensors are on {device}")
 
 
+def _fine(t: Tensor, types: dict) -> bool:
+    return t.is_cuda and t.dtype in types
+
+
 def _call(what: str, device: torch.device, fn, *args) -> None:
     """``fn(*args, stream)`` on ``device``'s current stream (the C ABI launches on the current device). The raw stream
     handle is asked for directly: a ``torch.cuda.Stream`` object costs as much host time as the launch."""
     index = device.index
-    if index == torch._C._cuda_getDevice():
-        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if index == _current_device():
+        status = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+            status = fn(*args, _raw_stream(index))
     if status:
         _native.check(status, what)
 
@@ -141,8 +147,9 @@ def scaled_embedding(tokens: Tensor, weight: Tensor, scale: float = 1.0, dtype: 
     ``tokens``: int32 or int64 of any shape; an id outside ``[0, V)`` gives a row of zeros and no gradient. ``weight``
     ``[V, C]``: float32, float16 or bfloat16. Differentiable in ``weight`` to every order; the gradient has its type and is
     summed in float32."""
-    _require(weight, "scaled_embedding", "weight", _DTYPES)
-    _require(tokens, "scaled_embedding", "tokens", _IDS, weight.device)
+    if not _fine(weight, _DTYPES) or not _fine(tokens, _IDS) or tokens.device != weight.device:
+        _require(weight, "scaled_embedding", "weight", _DTYPES)
+        _require(tokens, "scaled_embedding", "tokens", _IDS, weight.device)
     if weight.dim() != 2 or not weight.shape[0] or not weight.shape[1]:
         raise ValueError(f"scaled_embedding: weight must be [V, C], got {tuple(weight.shape)}")
     dtype = weight.dtype if dtype is None else dtype
@@ -311,7 +318,8 @@ class _RowDots(torch.autograd.Function):
 def expert_dispatch(x: Tensor, route: ExpertRoute) -> Tensor:
     """Each token's vector in the rows of its experts: ``[rows, C]`` with ``rows[route.row_of[t, k]] = x[t]`` and zeros in
     rows of no slot. ``x`` [*tokens, C] in float32, float16 or bfloat16; differentiable to every order."""
-    _require(x, "expert_dispatch", "x", _DTYPES, route.row_of.device)
+    if not _fine(x, _DTYPES) or x.device != route.row_of.device:
+        _require(x, "expert_dispatch", "x", _DTYPES, route.row_of.device)
     if x.dim() < 1 or x.shape[:-1] != route.row_of.shape[:-1] or not x.shape[-1]:
         raise ValueError(
             f"expert_dispatch: x must be [*{tuple(route.row_of.shape[:-1])}, C] for this route, got {tuple(x.shape)}"
@@ -326,11 +334,13 @@ def expert_combine(rows: Tensor, route: ExpertRoute, weights: Optional[Tensor] =
     None: ones), ``[*tokens, C]``, dropped slots adding nothing. ``rows`` [rows, C] in float32, float16 or bfloat16;
     ``weights`` [*tokens, K] (float32 or the rows' type are read as they are). The sum is float32 with one rounding.
     Differentiable in both to every order."""
-    _require(rows, "expert_combine", "rows", _DTYPES, route.row_of.device)
+    if not _fine(rows, _DTYPES) or rows.device != route.row_of.device:
+        _require(rows, "expert_combine", "rows", _DTYPES, route.row_of.device)
     if rows.dim() != 2 or rows.shape[0] != route.rows or not rows.shape[1]:
         raise ValueError(f"expert_combine: rows must be [{route.rows}, C] for this route, got {tuple(rows.shape)}")
     if weights is not None:
-        _require(weights, "expert_combine", "weights", _DTYPES, rows.device)
+        if not _fine(weights, _DTYPES) or weights.device != rows.device:
+            _require(weights, "expert_combine", "weights", _DTYPES, rows.device)
         if weights.shape != route.row_of.shape:
             raise ValueError(
                 f"expert_combine: weights must be {tuple(route.row_of.shape)} for this route, got {tuple(weights.shape)}"
@@ -441,9 +451,11 @@ def topk_distill_loss(logits: Tensor, teacher_ids: Tensor, teacher_logits: Tenso
     in ``logits``; the teacher and the weights are constants. A reduced loss keeps a gradient of the logits' size from the
     forward to the backward pass."""
     what = "topk_distill_loss"
-    _require(logits, what, "logits", _DTYPES)
-    _require(teacher_ids, what, "teacher_ids", _IDS, logits.device)
-    _require(teacher_logits, what, "teacher_logits", _DTYPES, logits.device)
+    if not (_fine(logits, _DTYPES) and _fine(teacher_ids, _IDS) and _fine(teacher_logits, _DTYPES)
+            and logits.device == teacher_ids.device == teacher_logits.device):  # fmt: skip
+        _require(logits, what, "logits", _DTYPES)
+        _require(teacher_ids, what, "teacher_ids", _IDS, logits.device)
+        _require(teacher_logits, what, "teacher_logits", _DTYPES, logits.device)
     if logits.dim() < 1 or teacher_ids.dim() < 1 or teacher_ids.shape[:-1] != logits.shape[:-1] or not logits.shape[-1]:
         raise ValueError(f"{what}: logits [..., V] and teacher_ids [..., K] must have the same rows, got "
                          f"{tuple(logits.shape)} and {tuple(teacher_ids.shape)}")  # fmt: skip
@@ -463,7 +475,8 @@ def topk_distill_loss(logits: Tensor, teacher_ids: Tensor, teacher_logits: Tenso
         if row_weight.shape != logits.shape[:-1]:
             raise ValueError(f"{what}: row_weight must be {tuple(logits.shape[:-1])}, got {tuple(row_weight.shape)}")
         row_weight = row_weight.to(torch.float32).contiguous()
-    ids, top = teacher_ids.contiguous(), teacher_logits.contiguous()
+    ids = teacher_ids if teacher_ids.is_contiguous() else teacher_ids.contiguous()
+    top = teacher_logits if teacher_logits.is_contiguous() else teacher_logits.contiguous()
     rows = ids.numel() // ids.shape[-1]
     factor = 1.0 / rows if reduction == "mean" and rows else 1.0
     reduced = reduction != "none"

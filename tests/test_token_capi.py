@@ -47,9 +47,10 @@ def test_embedding_refusals(lib):
     size = lib.ebr_scaled_embedding_grad_scratch_bytes
     assert size(0, 10, 8) == 0 and size(4, 0, 8) == 0
     assert size(4, 10, 8) == 0  # few tokens: one launch that keeps nothing
-    assert size(400, 10, 8) >= 2 * 1600 + 2 * 8 * 4  # sorted keys and positions, two partial sums
+    assert size(512, 10, 8) == 0 and size(512, 4000, 8) > 0 and size(128, 4000, 8) == 0
+    assert size(4000, 10, 8) >= 2 * 16000 + 2 * 8 * 4  # sorted keys and positions, two partial sums
     assert size(1 << 20, 1 << 17, 64) >= 4 * (1 << 22)  # two passes: both pairs of arrays
-    g = lambda **k: lib.ebr_scaled_embedding_grad(*{**dict(g=BF16, w=F32, i=1, n=400, V=10, C=8, s=1.0, ids=P, p=P, gs=8,
+    g = lambda **k: lib.ebr_scaled_embedding_grad(*{**dict(g=BF16, w=F32, i=1, n=4000, V=10, C=8, s=1.0, ids=P, p=P, gs=8,
                                                            dw=P, sc=P, b=1 << 20, st=None), **k}.values())  # fmt: skip
     assert g(b=0) == _native.ERR_SCRATCH and g(sc=None) == _native.ERR_SCRATCH and g(sc=P + 4) == _native.ERR_SCRATCH
     assert g(dw=P + 4) == _native.ERR_STRIDE and g(dw=None) == _native.ERR_NULL and g(p=None) == _native.ERR_NULL

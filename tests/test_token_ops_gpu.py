@@ -87,7 +87,7 @@ def test_embedding_lookup(n, v, c, wtype, otype):
 
 
 @pytest.mark.parametrize("gtype,wtype", [(a, b) for a in TYPES for b in TYPES])
-@pytest.mark.parametrize("n,v,c", [(1, 1, 1), (81, 10, 512), (128, 2, 33), (129, 2, 33), (100, 3001, 771), (3000, 2, 33), (1000, 1023, 64), (1003, 1024, 771),
+@pytest.mark.parametrize("n,v,c", [(1, 1, 1), (81, 10, 512), (128, 2, 33), (512, 3, 520), (513, 3, 520), (100, 3001, 771), (129, 3001, 771), (3000, 2, 33), (1000, 1023, 64), (1003, 1024, 771),
                                    (6000, 5000, 72)])
 def test_embedding_gradient(n, v, c, gtype, wtype):
     from ebr_b200.token_ops import scaled_embedding
