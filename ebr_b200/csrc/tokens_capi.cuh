@@ -293,9 +293,10 @@ bool grad_by_few(int64_t n, int64_t V, int64_t C) {
 constexpr int64_t kMaxVocabulary = int64_t{1} << 19;
 constexpr int kMaxEntries = 1024;
 
-// Rows of a few logits take four lanes each, rows of up to kWarpRowBytes a warp, longer ones a ring of chunks: bfloat16 at
-// 2.1 GB of logits and gradient, a warp takes 0.53 ms at V = 8,192 (the ring 0.72) and 0.57 at 16,384 (0.60).
-constexpr int64_t kWarpRowBytes = 16 * 1024;
+// Rows of a few logits take four lanes each, rows of up to kWarpRowBytes a warp (half as much where there are not rows enough
+// to fill the GPU so), longer ones a ring of chunks. bfloat16, 2.1 GB of logits and gradient: a warp takes 0.52 ms at
+// V = 8,192 (the ring 0.72) and 0.57 at 16,384 (0.60).
+constexpr int64_t kWarpRowBytes = 32 * 1024;
 
 bool distill_few(int64_t V, int64_t K) { return V <= 32 && K <= 32; }
 
@@ -309,8 +310,8 @@ int launch_distill_few(const ebr::distill::Args& a, cudaStream_t st) {
 }
 
 template <typename T>
-bool distill_by_warp(int64_t V) {
-  return V * static_cast<int64_t>(sizeof(T)) <= kWarpRowBytes;
+bool distill_by_warp(int64_t N, int64_t V) {
+  return V * static_cast<int64_t>(sizeof(T)) <= (N >= 256 ? kWarpRowBytes : kWarpRowBytes / 2);
 }
 
 template <typename T, bool kStats>
@@ -374,7 +375,7 @@ int64_t row_granules(int64_t V) {
 template <typename T>
 int launch_distill(int device, const ebr::distill::Args& a, cudaStream_t st) {
   if (distill_few(a.V, a.K)) return launch_distill_few<T, true>(a, st);
-  if (distill_by_warp<T>(a.V)) return launch_distill_warp<T, true>(a, st);
+  if (distill_by_warp<T>(a.N, a.V)) return launch_distill_warp<T, true>(a, st);
   const int64_t total = row_granules<T>(a.V);
   int slices = 1;
   while (slices < ebr::distill::kMaxSlices && a.N * slices < 2 * sm_count(device) && (total + slices - 1) / slices > 256)
@@ -391,7 +392,7 @@ int launch_distill(int device, const ebr::distill::Args& a, cudaStream_t st) {
 template <typename T>
 int launch_distill_grad(int device, const ebr::distill::Args& a, cudaStream_t st) {
   if (distill_few(a.V, a.K)) return launch_distill_few<T, false>(a, st);
-  if (distill_by_warp<T>(a.V)) return launch_distill_warp<T, false>(a, st);
+  if (distill_by_warp<T>(a.N, a.V)) return launch_distill_warp<T, false>(a, st);
   constexpr int kThreads = 256;
   const int64_t total = row_granules<T>(a.V);
   const int slices = static_cast<int>((total + 4095) / 4096);
