@@ -5,6 +5,11 @@
 //
 // Exponentials are 2^((s - largest) * log2(e) / tau): the difference is taken before the scaling, so the exponent of a
 // term that counts is exact to a few ulp, and the largest term is exactly 1.
+//
+// Measured, bfloat16, 64 entries, loss and gradient in one pass: 4,096 rows of 131,072 take 444 us (4.8 TB/s of logits and
+// gradient; the loss alone 202, 5.3 TB/s; the gradient alone 348, 6.2 TB/s), 16,384 of 32,768 504 us, 65,536 of 8,192 515 us,
+// 131,072 of 4,096 (16 entries) 394 us (5.5 TB/s). The one-pass kernel is bound by latency, issue and the exponential
+// unit together (58 and 54 % busy with sixteen warps on an SM at 463 us); the rings leave room for 24.
 #pragma once
 
 #include "../../include/ebr_tokens.h"

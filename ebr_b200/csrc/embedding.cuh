@@ -6,6 +6,11 @@
 // equal ids of its chunk for 32 vectors of columns. A run that lies in one chunk goes straight to dW; a run that crosses
 // chunks leaves one float32 partial sum per chunk, which a second kernel adds in chunk order. A table of ten rows
 // under 62,208 tokens (runs of thousands) and one of 131,072 rows (runs of one or two) take the same path.
+//
+// Measured: the lookup of 16,384 bfloat16 tokens of 2,048 columns 16.5 us (8.1 TB/s of its rows and output, some of it from
+// L2), of 62,208 board tokens of 512 columns from a float32 table 17 us (3.7 TB/s: the table's rows come from L1 as 32 bytes
+// a lane); the gradients of the same 111 us (5.5 TB/s; 74 of it zero the table, beside the sort) and 31 us (chunks 17, the
+// join 8, the sort 7: the latency of four short kernels).
 #pragma once
 
 #include <type_traits>

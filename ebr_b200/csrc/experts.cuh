@@ -9,6 +9,11 @@
 // in flight at once; where the tokens are few, several warps
 // (blockIdx.y) share a token's columns. The rows' numbers and weights of up to 32 slots sit in the lanes. Rows of no slot are zeroed by
 // further blocks of the same launch.
+//
+// Measured, bfloat16: 16,384 tokens of 2,048 columns to eight of 64 experts: dispatch 107 us (5.7 TB/s), combine 96 (6.3),
+// combine's gradients 189 (6.1); the board batch (62,208 of 512, two of eight): 39, 39 and 62 us (4.8 to 5.1 TB/s, a row of
+// one kilobyte being two accesses of a warp). Rows of an odd number of 16-bit elements go two bytes a lane: 30,000 tokens of
+// 1,001 to four of 32 take 74, 105 and 144 us (2.8 to 4.1 TB/s); reading them as shifted 16-byte windows was slower.
 #pragma once
 
 #include "embedding.cuh"

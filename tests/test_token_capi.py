@@ -41,7 +41,7 @@ def test_embedding_refusals(lib):
     assert f(w=F64) == _native.ERR_DTYPE and f(o=9) == _native.ERR_DTYPE and f(i=2) == _native.ERR_DTYPE
     assert f(V=0) == _native.ERR_SHAPE and f(C=0) == _native.ERR_SHAPE and f(n=-1) == _native.ERR_SHAPE
     assert f(n=1 << 30) == _native.ERR_SHAPE and f(V=1 << 30) == _native.ERR_SHAPE
-    assert f(ws=-8) == _native.ERR_STRIDE
+    assert f(ws=-8) == _native.ERR_STRIDE and f(ids=P + 4) == _native.ERR_STRIDE
     assert f(ids=None) == _native.ERR_NULL and f(p=None) == _native.ERR_NULL and f(out=None) == _native.ERR_NULL
     assert f(n=0, ids=None, p=None, out=None) == _native.OK
     size = lib.ebr_scaled_embedding_grad_scratch_bytes
@@ -90,6 +90,7 @@ def test_distillation_refusals(lib):
                 dict(tau=float("nan")), dict(N=-1)):  # fmt: skip
         assert f(**bad) == _native.ERR_SHAPE, bad
     assert f(xs=-1) == _native.ERR_STRIDE and f(g=P, gs=99) == _native.ERR_STRIDE
+    assert f(ids=P + 4) == _native.ERR_STRIDE and f(s=P + 4) == _native.ERR_STRIDE
     for bad in (dict(x=None), dict(ids=None), dict(top=None), dict(l=None), dict(s=None)):
         assert f(**bad) == _native.ERR_NULL, bad
     assert f(N=0, x=None, ids=None, top=None, l=None, s=None) == _native.OK

@@ -129,6 +129,31 @@ def test_embedding_gradient_sort_paths(n, v, c, kind):
     assert_within(dw, ref, (count + 2) * E * mag + U[torch.float32] * ref.abs())
 
 
+def test_embedding_gradient_of_a_large_table_replays_as_a_cuda_graph():
+    """The zeroing that runs beside the sort keeps its order in a graph: other tokens, the same buffers, several replays."""
+    from ebr_b200.token_ops import scaled_embedding
+
+    v, c, n = 1 << 20, 24, 20000
+    tokens, g = randint(-1, v, (n,), seed=1), rand(n, c, seed=2)
+    w = torch.zeros(v, c, device=DEV, requires_grad=True)
+
+    def step():
+        return torch.autograd.grad(scaled_embedding(tokens, w), w, g)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dw = step()
+    for seed in (3, 4, 5):
+        tokens.copy_(randint(-1, v, (n,), seed=seed))
+        graph.replay()
+        assert torch.equal(dw, step())
+
+
 def test_embedding_ids_far_outside_the_table_and_empty_inputs():
     from ebr_b200.token_ops import scaled_embedding
 
