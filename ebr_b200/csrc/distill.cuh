@@ -1,15 +1,16 @@
 // distill.cuh: the distillation loss on a teacher's top logits and its gradient (formulas: include/ebr_tokens.h).
 //
-// Short rows take a few lanes each; long ones a cluster that holds the row in shared memory. The gradient of the logits
-// that the teacher names is written after the dense pass.
+// A row of a few logits takes four lanes, one of up to 32 KB a warp, a longer one a CTA or a cluster with the row in
+// a shared-memory ring. The gradient of the logits that the teacher names is written after the dense pass.
 //
-// Exponentials are 2^((s - largest) * log2(e) / tau): the difference is taken before the scaling, so the exponent of a
-// term that counts is exact to a few ulp, and the largest term is exactly 1.
+// Exponentials are 2^((s - largest) * log2(e) / tau): the difference is taken before the scaling, so the exponent of
+// a term that counts is exact to a few ulp, and the largest term is exactly 1.
 //
-// Measured, bfloat16, 64 entries, loss and gradient in one pass: 4,096 rows of 131,072 take 444 us (4.8 TB/s of logits and
-// gradient; the loss alone 202, 5.3 TB/s; the gradient alone 348, 6.2 TB/s), 16,384 of 32,768 504 us, 65,536 of 8,192 515 us,
-// 131,072 of 4,096 (16 entries) 394 us (5.5 TB/s). The one-pass kernel is bound by latency, issue and the exponential
-// unit together (58 and 54 % busy with sixteen warps on an SM at 463 us); the rings leave room for 24.
+// Measured, bfloat16, 64 entries, loss and gradient in one pass: 4,096 rows of 131,072 take 444 us (4.8 TB/s of
+// logits and gradient; the loss alone 202, 5.3 TB/s; the gradient alone 348, 6.2 TB/s), 16,384 of 32,768 504 us,
+// 65,536 of 8,192 515 us, 131,072 of 4,096 (16 entries) 394 us (5.5 TB/s). The one-pass kernel is bound by latency,
+// issue and the exponential unit together (58 and 54 % busy with sixteen warps on an SM at 463 us); the rings leave
+// room for 24.
 #pragma once
 
 #include "../../include/ebr_tokens.h"
@@ -68,8 +69,8 @@ __device__ __forceinline__ float2 exp2_pair(float2 v, float base, float scale) {
 __device__ __forceinline__ float2 add2(float2 a, float2 b) { return make_float2(a.x + b.x, a.y + b.y); }
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) { return make_float2(a.x * b.x, a.y * b.y); }
 
-// A 16-byte granule of logits as pairs of floats, the larger elements of two granules place by place and the largest of
-// one (NaN passed over), and pairs back to a granule.
+// A 16-byte granule of logits as pairs of floats, the larger elements of two granules place by place and the largest
+// of one (NaN passed over), and pairs back to a granule.
 template <typename T>
 struct Granule;
 template <>
@@ -175,8 +176,8 @@ __device__ __forceinline__ float exp2_sum(const uint4& g, float base, float scal
   return v[0].x + v[0].y;
 }
 
-// A maximum and the sum of 2^((v - maximum) * scale). Maxima pass NaN over (an instruction less per element); a NaN makes
-// the sum NaN, and with it the row's loss and gradient, all the same.
+// A maximum and the sum of 2^((v - maximum) * scale). Maxima pass NaN over (an instruction less per element); a NaN
+// makes the sum NaN, and with it the row's loss and gradient, all the same.
 struct Stat {
   float m = -INFINITY, s = 0.f;
   __device__ __forceinline__ float base() const { return m == -INFINITY ? 0.f : -m; }  // terms of -inf are 0, not NaN
@@ -186,7 +187,8 @@ struct Stat {
   }
 };
 
-// A row that does not count (no entry of the teacher, or weight 0) has this sum among the statistics: no other row can.
+// A row that does not count (no entry of the teacher, or weight 0) has this sum among the statistics: no other row
+// can.
 __device__ __forceinline__ float2 no_row() { return make_float2(0.f, INFINITY); }
 
 // Sum over the kLanes consecutive lanes of a group.
@@ -390,7 +392,8 @@ __device__ __forceinline__ void bulk_wait_read() {
 // What the waits of distill_row_kernel record when they run out; they go on then, so that nothing hangs.
 constexpr int kFullWaitSite = 7001, kEmptyWaitSite = 7002, kExchangeWaitSite = 7003;
 
-// The statistics of one warp, and their announcement on an mbarrier, in the shared memory of CTA `rank` of the cluster.
+// The statistics of one warp, and their announcement on an mbarrier, in the shared memory of CTA `rank` of the
+// cluster.
 __device__ __forceinline__ void push_stat(float2* slot, uint64_t* bar, uint32_t rank, float m, float s) {
   asm volatile(
       "{\n\t.reg .b32 a, b;\n\t"
@@ -466,15 +469,16 @@ __global__ void __launch_bounds__(256) distill_weights_kernel(const __grid_const
   if ((threadIdx.x & 31) == 0) weights[n] = w;
 }
 
-// The dense part of long rows: the statistics, and grad = c_n q where a.grad is set, so that the logits cross HBM once.
-// CTA `slice` of a cluster of `slices` (one, unless the rows are few) serves a slice of the row's granules, in chunks of
-// kU granules for each lane, which pass through a ring of `slots` chunks in shared memory. The last warp loads (TMA); the
-// others reduce a row's chunks in order, exchange their statistics, and then turn the chunks into the gradient in place
-// and store them (TMA), each warp its own part of a chunk, so that within a row the warps meet only for the exchange.
-// The last chunks of a row stay in the ring between the two passes; only what does not fit is loaded again, soon after
-// its first reading, from L2. While a row is in its second pass, the freed slots already take the next row.
-// The chunks are freed in the order in which they were loaded, so the ring needs no bookkeeping but two counters.
-// What needs the teacher's entries is left to distill_entries_kernel: here each warp of each CTA would pay for it.
+// The dense part of long rows: the statistics, and grad = c_n q where a.grad is set, so that the logits cross HBM
+// once. CTA `slice` of a cluster of `slices` (one, unless the rows are few) serves a slice of the row's granules, in
+// chunks of kU granules for each lane, which pass through a ring of `slots` chunks in shared memory. The last warp
+// loads (TMA); the others reduce a row's chunks in order, exchange their statistics, and then turn the chunks into
+// the gradient in place and store them (TMA), each warp its own part of a chunk, so that within a row the warps meet
+// only for the exchange. The last chunks of a row stay in the ring between the two passes; only what does not fit is
+// loaded again, soon after its first reading, from L2. While a row is in its second pass, the freed slots already
+// take the next row. The chunks are freed in the order in which they were loaded, so the ring needs no bookkeeping
+// but two counters. What needs the teacher's entries is left to distill_entries_kernel: here each warp of each CTA
+// would pay for it.
 constexpr int kMaxSlots = 16;
 
 template <typename T, int kWarps, int kU>
@@ -490,8 +494,8 @@ __global__ void __launch_bounds__(kWarps * 32 + 32) distill_row_kernel(const __g
   const int slice = static_cast<int>(blockIdx.x) % slices;
   const int rows = static_cast<int>(a.N), step = static_cast<int>(gridDim.x) / slices;
   uint4* ring = reinterpret_cast<uint4*>(smem);
-  // This CTA's whole granules of a row: `count` of them from element `begin` on. The row's ragged ends, at most two of
-  // them in a slice, belong to lanes 0 and 1 of warp 0.
+  // This CTA's whole granules of a row: `count` of them from element `begin` on. The row's ragged ends, at most two
+  // of them in a slice, belong to lanes 0 and 1 of warp 0.
   struct Slice {
     const T* row;
     int begin, count, chunks, kept;
@@ -694,52 +698,7 @@ __global__ void __launch_bounds__(kWarps * 32 + 32) distill_row_kernel(const __g
   }
 }
 
-// The dense part of the gradient alone, from the forward's statistics: blocks walk (row, slice) items.
-template <typename T, int kThreads>
-__global__ void __launch_bounds__(kThreads) distill_grad_kernel(const __grid_constant__ Args a, int slices,
-                                                                int slice_granules) {
-  constexpr int kAhead = 4;
-  if (a.unless_one && a.upstream[0] == 1.f) return;
-  for (int64_t item = blockIdx.x; item < a.N * slices; item += gridDim.x) {
-    const int64_t n = item / slices;
-    const int slice = static_cast<int>(item % slices);
-    const float m = a.stats[2 * n], sum = a.stats[2 * n + 1];
-    T* grad = static_cast<T*>(a.grad) + n * a.grad_stride;
-    const Granules<T> row(static_cast<const T*>(a.logits) + n * a.logits_stride, a.V), out(grad, a.V);
-    if (sum == INFINITY) {  // no_row
-      const int span = (out.count() + slices - 1) / slices;
-      zero_granules(out, min(out.count(), slice * span), min(out.count(), (slice + 1) * span), kThreads, grad);
-      continue;
-    }
-    const int lo = min(row.count(), slice * slice_granules), hi = min(row.count(), lo + slice_granules);
-    const float mult = a.factor * a.upstream[n * a.upstream_stride] * (a.row_weight ? a.row_weight[n] : 1.f) * a.tau / sum;
-    const bool same = row.phase == out.phase;
-    for (int g0 = lo + threadIdx.x; g0 < hi; g0 += kAhead * kThreads) {
-      uint4 v[kAhead];
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int g = g0 + u * kThreads;
-        if (g >= hi) continue;
-        if (row.whole(g))
-          v[u] = *reinterpret_cast<const uint4*>(row.row + row.first(g));
-        else
-          v[u] = ragged(row, g);
-      }
-#pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int g = g0 + u * kThreads;
-        if (g >= hi) continue;
-        const uint4 o = grad_granule<T>(v[u], m, a.exp2_scale, mult);
-        if (same && row.whole(g))
-          *reinterpret_cast<uint4*>(grad + row.first(g)) = o;
-        else
-          store_elements<T>(o, row.first(g), row.V, grad);
-      }
-    }
-  }
-}
-
-// ------------------------------------------------------------------------------------------------ the teacher's entries
+// --------------------------------------------------------------------------------------------- the teacher's entries
 
 // One row's entries, by one warp, in its shared memory: ids, logits that become probabilities, and a table of bits.
 struct Entries {
@@ -790,9 +749,9 @@ struct Entries {
     }
     return kLoss ? lanes_sum<32>(loss) : 0.f;
   }
-  // The gradient of the logits that they name, over what the dense pass wrote. Entries that repeat an id share the sum of
-  // their p: the table finds the entries that may be such (two ids can have one bit), and the warp adds up each of those
-  // ids' p in the entries' order, so that the rest (nearly all) cost nothing.
+  // The gradient of the logits that they name, over what the dense pass wrote. Entries that repeat an id share the
+  // sum of their p: the table finds the entries that may be such (two ids can have one bit), and the warp adds up
+  // each of those ids' p in the entries' order, so that the rest (nearly all) cost nothing.
   template <typename T>
   __device__ __forceinline__ void store(const Args& a, const T* row, float m, float inv_sum, float coef, T* grad) {
     const unsigned bits = 32u * static_cast<unsigned>(a.K);
@@ -822,6 +781,65 @@ struct Entries {
   }
 };
 
+// The gradient alone, from the forward's statistics: its dense part, blocks walking over (row, slice) items; with
+// kEntries (whole rows: one slice) the entries' part too, by the block's first warp, which keeps to one launch the
+// check that usually ends it.
+template <typename T, int kThreads, bool kEntries>
+__global__ void __launch_bounds__(kThreads) distill_grad_kernel(const __grid_constant__ Args a, int slices,
+                                                                int slice_granules) {
+  constexpr int kAhead = 4;
+  extern __shared__ __align__(16) unsigned char smem[];
+  if (a.unless_one && a.upstream[0] == 1.f) return;
+  for (int64_t item = blockIdx.x; item < a.N * slices; item += gridDim.x) {
+    const int64_t n = item / slices;
+    const int slice = static_cast<int>(item % slices);
+    const float m = a.stats[2 * n], sum = a.stats[2 * n + 1];
+    T* grad = static_cast<T*>(a.grad) + n * a.grad_stride;
+    const Granules<T> row(static_cast<const T*>(a.logits) + n * a.logits_stride, a.V), out(grad, a.V);
+    if (sum == INFINITY) {  // no_row
+      const int span = (out.count() + slices - 1) / slices;
+      zero_granules(out, min(out.count(), slice * span), min(out.count(), (slice + 1) * span), kThreads, grad);
+      continue;
+    }
+    const int lo = min(row.count(), slice * slice_granules), hi = min(row.count(), lo + slice_granules);
+    const float coef = a.factor * a.upstream[n * a.upstream_stride] * (a.row_weight ? a.row_weight[n] : 1.f) * a.tau;
+    const float mult = coef / sum;
+    const bool same = row.phase == out.phase;
+    for (int g0 = lo + threadIdx.x; g0 < hi; g0 += kAhead * kThreads) {
+      uint4 v[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int g = g0 + u * kThreads;
+        if (g >= hi) continue;
+        if (row.whole(g))
+          v[u] = *reinterpret_cast<const uint4*>(row.row + row.first(g));
+        else
+          v[u] = ragged(row, g);
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int g = g0 + u * kThreads;
+        if (g >= hi) continue;
+        const uint4 o = grad_granule<T>(v[u], m, a.exp2_scale, mult);
+        if (same && row.whole(g))
+          *reinterpret_cast<uint4*>(grad + row.first(g)) = o;
+        else
+          store_elements<T>(o, row.first(g), row.V, grad);
+      }
+    }
+    if constexpr (kEntries) {
+      __syncthreads();  // the dense part is complete
+      if (threadIdx.x < 32) {
+        Entries e(smem, a.K, threadIdx.x);
+        e.read(a, n);
+        e.normalise(a);
+        e.template finish<T, false>(a, row.row, m, 0.f);
+        e.template store<T>(a, row.row, m, 1.f / sum, coef, grad);
+      }
+    }
+  }
+}
+
 // What the entries add to long rows: the loss (kLoss), and the gradient of the logits that they name (a.grad set).
 constexpr int kEntryWarps = 4;
 
@@ -847,10 +865,10 @@ __global__ void __launch_bounds__(kEntryWarps * 32) distill_entries_kernel(const
   e.store<T>(a, row, st.x, 1.f / st.y, a.factor * up * weight * a.tau, static_cast<T*>(a.grad) + n * a.grad_stride);
 }
 
-// ------------------------------------------------------------------------------------------------ rows of middling length
+// ------------------------------------------------------------------------------------------- rows of middling length
 
-// A warp serves a row, all of it: no barrier stands between the readings, and a row of some KB is still in L1 or L2 at its
-// second one. kStats: find the statistics and the loss, else read the statistics.
+// A warp serves a row, all of it: no barrier stands between the readings, and a row of some KB is still in L1 or L2
+// at its second one. kStats: find the statistics and the loss, else read the statistics.
 constexpr int kMidWarps = 4;
 
 template <typename T, bool kStats>
@@ -880,8 +898,8 @@ __global__ void __launch_bounds__(kMidWarps * 32) distill_warp_kernel(const __gr
     return;
   }
   const Granules<T> row(static_cast<const T*>(a.logits) + n * a.logits_stride, a.V);
-  // The whole granules [begin, end) go by vectors; the row's ragged ends, at most two, belong to lanes 0 and 1. A lane past
-  // the last whole granule reads that one again and drops it: no branch stands between the loads.
+  // The whole granules [begin, end) go by vectors; the row's ragged ends, at most two, belong to lanes 0 and 1. A
+  // lane past the last whole granule reads that one again and drops it: no branch stands between the loads.
   const int begin = row.first_whole(), end = row.end_whole();
   const int edge = row.ragged_end(lane);
   const uint4 ragged_end = edge >= 0 ? ragged(row, edge) : Granule<T>::none();

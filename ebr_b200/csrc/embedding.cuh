@@ -1,16 +1,17 @@
-// embedding.cuh: the scaled embedding out[t] = scale * W[id_t] and its gradient dW[v] = scale * sum_{t: id_t = v} g[t].
+// embedding.cuh: the scaled embedding out[t] = scale * W[id_t] and its gradient dW[v] = scale * sum_{t: id_t = v}
+// g[t].
 //
 // Both are bound by HBM: the lookup writes n rows (and reads the distinct rows of W), the gradient reads n rows of g
-// and writes the whole table. The gradient needs no atomics: the tokens are sorted by id (key_sort.cuh), so the rows of
-// one id are neighbours in the sorted order. The sorted tokens are cut into chunks of R rows; a warp sums the runs of
-// equal ids of its chunk for 32 vectors of columns. A run that lies in one chunk goes straight to dW; a run that crosses
-// chunks leaves one float32 partial sum per chunk, which a second kernel adds in chunk order. A table of ten rows
-// under 62,208 tokens (runs of thousands) and one of 131,072 rows (runs of one or two) take the same path.
+// and writes the whole table. The gradient needs no atomics: the tokens are sorted by id (key_sort.cuh), so the rows
+// of one id are neighbours in the sorted order. The sorted tokens are cut into chunks of R rows; a warp sums the runs
+// of equal ids of its chunk for 32 vectors of columns. A run that lies in one chunk goes straight to dW; a run that
+// crosses chunks leaves one float32 partial sum per chunk, which a second kernel adds in chunk order. A table of ten
+// rows under 62,208 tokens (runs of thousands) and one of 131,072 rows (runs of one or two) take the same path.
 //
-// Measured: the lookup of 16,384 bfloat16 tokens of 2,048 columns 16.5 us (8.1 TB/s of its rows and output, some of it from
-// L2), of 62,208 board tokens of 512 columns from a float32 table 17 us (3.7 TB/s: the table's rows come from L1 as 32 bytes
-// a lane); the gradients of the same 111 us (5.5 TB/s; 74 of it zero the table, beside the sort) and 31 us (chunks 17, the
-// join 8, the sort 7: the latency of four short kernels).
+// Measured: the lookup of 16,384 bfloat16 tokens of 2,048 columns 16.5 us (8.1 TB/s of its rows and output, some of
+// it from L2), of 62,208 board tokens of 512 columns from a float32 table 17 us (3.7 TB/s: the table's rows come from
+// L1 as 32 bytes a lane); the gradients of the same 111 us (5.5 TB/s; 74 of it zero the table, beside the sort) and
+// 31 us (chunks 17, the join 8, the sort 7: the latency of four short kernels).
 #pragma once
 
 #include <type_traits>
@@ -43,8 +44,8 @@ struct Word<16> {
   using type = uint4;
 };
 
-// V elements of T as they are in memory (at most 16 bytes), and as floats. The 16-bit types are converted two at a time
-// from whole words.
+// V elements of T as they are in memory (at most 16 bytes), and as floats. The 16-bit types are converted two at a
+// time from whole words.
 template <typename T, int V>
 struct Raw {
   using W = typename Word<V * sizeof(T)>::type;
@@ -119,9 +120,9 @@ __device__ __forceinline__ void store_f(T* p, const float (&in)[V]) {
 
 // ------------------------------------------------------------------------------------------------ lookup
 
-// A warp writes up to 32 consecutive tokens' parts of kU * 32 vectors of columns (blockIdx.y picks them): its lanes read
-// the ids at once, and kLookupAhead / kU rows are in flight, so that the chain id -> row -> store is paid once for many
-// rows. Whole rows by one warp where they fit: neighbouring rows are then written as one stretch.
+// A warp writes up to 32 consecutive tokens' parts of kU * 32 vectors of columns (blockIdx.y picks them): its lanes
+// read the ids at once, and kLookupAhead / kU rows are in flight, so that the chain id -> row -> store is paid once
+// for many rows. Whole rows by one warp where they fit: neighbouring rows are then written as one stretch.
 constexpr int kLookupWarps = 4, kLookupAhead = 4;
 
 template <typename TW, typename TO, int V, int kU>
@@ -164,8 +165,8 @@ __global__ void __launch_bounds__(kLookupWarps * 32) lookup_kernel(IdSource src,
 
 constexpr int kGradWarps = 8;
 
-// part[chunk][0]: the sum of the run that the chunk starts in the middle of; part[chunk][1]: of the run that starts in
-// the chunk and goes on in the next. Rows of C floats.
+// part[chunk][0]: the sum of the run that the chunk starts in the middle of; part[chunk][1]: of the run that starts
+// in the chunk and goes on in the next. Rows of C floats.
 template <typename TG, typename TW, int V>
 __global__ void __launch_bounds__(kGradWarps * 32) grad_chunk_kernel(int n, int range, int64_t C, int R,
                                                                      const int* __restrict__ key,
@@ -246,8 +247,9 @@ __global__ void __launch_bounds__(kGradWarps * 32) grad_chunk_kernel(int n, int 
 }
 
 // Runs that cross chunks. A block looks at the ends of kJoinChunks chunks, a warp at one of them: where the run at a
-// chunk's end started in that chunk and goes on, its partials are added in chunk order. A run of a few chunks is added by
-// its warp, 32 vectors of four columns; a long one by the whole block, every warp taking every kJoinWarps-th partial.
+// chunk's end started in that chunk and goes on, its partials are added in chunk order. A run of a few chunks is
+// added by its warp, 32 vectors of four columns; a long one by the whole block, every warp taking every kJoinWarps-th
+// partial.
 constexpr int kJoinWarps = 32, kJoinChunks = 32, kJoinShort = 16;
 
 template <typename TW>
@@ -348,8 +350,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32) grad_join_kernel(int n, int r
   }
 }
 
-// Few tokens: kShare warps own a table row's part and go through all ids themselves, each through its stretch of them, adding
-// the rows of their own in their order. No sort, no zeroing, no joining: one launch, where the launches are the cost.
+// Few tokens: kShare warps own a table row's part and go through all ids themselves, each through its stretch of
+// them, adding the rows of their own in their order. No sort, no zeroing, no joining: one launch, where the launches
+// are the cost.
 template <typename TG, typename TW, int V, int kShare>
 __global__ void __launch_bounds__(kGradWarps * 32) grad_few_kernel(IdSource src, int n, int64_t C,
                                                                    const TG* __restrict__ g, int64_t g_stride,

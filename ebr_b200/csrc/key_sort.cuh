@@ -1,14 +1,14 @@
 // key_sort.cuh: a stable sort of small integer keys with their positions, the common first step of the embedding's
-// gradient (tokens by id) and of the expert route (slots by expert). Least-significant-digit counting passes of at most
-// kMaxDigitBits bits: every key's place is  start of its digit + keys of that digit before it.
+// gradient (tokens by id) and of the expert route (slots by expert). Least-significant-digit counting passes of at
+// most kMaxDigitBits bits: every key's place is  start of its digit + keys of that digit before it.
 //
-// Ranking inside a block: each warp owns a contiguous stretch of keys and walks it 32 at a time. __match_any_sync gives
-// the lanes that hold the same digit, so a key's rank in its warp is the warp's running count of the digit plus the
-// earlier lanes of the match; the counts of the block's warps are then scanned per digit. The order of equal keys never
-// depends on timing, so everything built on it is deterministic.
+// Ranking inside a block: each warp owns a contiguous stretch of keys and walks it 32 at a time. __match_any_sync
+// gives the lanes that hold the same digit, so a key's rank in its warp is the warp's running count of the digit plus
+// the earlier lanes of the match; the counts of the block's warps are then scanned per digit. The order of equal keys
+// never depends on timing, so everything built on it is deterministic.
 //
-// Bound by latency, not by bytes (a million bytes of ids): 162 slots take 4.5 us and 18,006 take 6.5 in one cluster, 124,416
-// take 6.9 in two kernels over the whole GPU, replayed from a CUDA graph.
+// Bound by latency, not by bytes (a million bytes of ids): 162 slots take 4.5 us and 18,006 take 6.5 in one cluster,
+// 124,416 take 6.9 in two kernels over the whole GPU, replayed from a CUDA graph.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -71,8 +71,8 @@ struct SmallZero {
 
 // ------------------------------------------------------------------------------------------------ block-level parts
 
-// Ranks the block's keys [begin, begin + kItems * 32 of each warp) among the block's equal digits: dig / rank of item j
-// of this thread (dig = -1 past the end), and after the call counts[w * digits + d] = keys of digit d in the warps
+// Ranks the block's keys [begin, begin + kItems * 32 of each warp) among the block's equal digits: dig / rank of item
+// j of this thread (dig = -1 past the end), and after the call counts[w * digits + d] = keys of digit d in the warps
 // before w, totals[d] = keys of digit d in the block. Keys with digit >= digits get no rank (dig = -1).
 template <int kItems, typename KeyFn>
 __device__ __forceinline__ void rank_block(int64_t warp_begin, int64_t warp_end, int digits, KeyFn key_of,
@@ -138,8 +138,8 @@ __device__ __forceinline__ int block_exclusive(int v, int* warp_sums, int* total
   return x - v + warp_sums[warp];
 }
 
-// Rows of no slot, and the offsets: the part of a route that does not depend on single slots. digit_start / digit_total
-// [experts] are shared arrays; `part` of `parts` blocks share the row walk.
+// Rows of no slot, and the offsets: the part of a route that does not depend on single slots. digit_start /
+// digit_total [experts] are shared arrays; `part` of `parts` blocks share the row walk.
 __device__ __forceinline__ void finish_route(const RouteOut& r, const int* digit_start, const int* digit_total,
                                              int live, int part, int parts) {
   if (part == 0) {
@@ -185,9 +185,9 @@ struct ClusterSort {
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// Zeros a byte range, kZeroPiece bytes to a block (contiguous pieces: 7.1 TB/s on 537 MB; a grid-stride walk 5.9). It is
-// launched behind the cluster sort, which does not touch the range, to run beside it on the SMs that the sort leaves
-// free; the last block ends only after the sort, so whatever follows in the stream finds both done.
+// Zeros a byte range, kZeroPiece bytes to a block (contiguous pieces: 7.1 TB/s on 537 MB; a grid-stride walk 5.9). It
+// is launched behind the cluster sort, which does not touch the range, to run beside it on the SMs that the sort
+// leaves free; the last block ends only after the sort, so whatever follows in the stream finds both done.
 constexpr int64_t kZeroPiece = 128 * 1024;
 
 __global__ void __launch_bounds__(1024) zero_kernel(char* p, int64_t bytes) {
@@ -287,8 +287,8 @@ __global__ void __launch_bounds__(kSortThreads, 1) cluster_sort_kernel(const __g
 // ------------------------------------------------------------------------------------------------ whole grid
 
 // For more keys: per pass, one block per tile of kSortThreads * kItems keys counts its digits, and one block per tile
-// ranks and places its keys. With up to kMaxTiles tiles the second kernel adds up the tiles before its own itself; with
-// more, a kernel between the two scans the counts.
+// ranks and places its keys. With up to kMaxTiles tiles the second kernel adds up the tiles before its own itself;
+// with more, a kernel between the two scans the counts.
 constexpr int kMaxTiles = 256;
 
 struct GridSort {

@@ -1,6 +1,6 @@
 // tokens_capi.cuh: the C ABI of include/ebr_tokens.h (included at the end of capi.cu, after layers_capi.cuh, whose
-// dtype and alignment helpers it uses). Validates arguments, picks the access width and launch shape, and launches the
-// kernels of key_sort.cuh, embedding.cuh, experts.cuh and distill.cuh on the caller's stream.
+// dtype and alignment helpers it uses). Validates arguments, picks the access width and launch shape, and launches
+// the kernels of key_sort.cuh, embedding.cuh, experts.cuh and distill.cuh on the caller's stream.
 #pragma once
 
 #include "../../include/ebr_tokens.h"
@@ -85,13 +85,14 @@ int with_width(int v, Fn&& fn) {
 
 // ------------------------------------------------------------------------------------------------ sort
 
-// Keys that one cluster of 16 CTAs ranks in registers, and those up to which it is used even where nothing runs beside
-// it: 18,006 slots take 8.7 us in a cluster; 124,416 take 15.6 there and 7.0 in two kernels over the whole GPU.
+// Keys that one cluster of 16 CTAs ranks in registers, and those up to which it is used even where nothing runs
+// beside it: 18,006 slots take 8.7 us in a cluster; 124,416 take 15.6 there and 7.0 in two kernels over the whole
+// GPU.
 constexpr int64_t kClusterKeys = 16 * int64_t{ebr::keysort::kSortThreads} * 16;
 constexpr int64_t kClusterAlone = 32 * 1024;
 
-// Bytes of zeros from which the sort in one cluster hides behind the zeroing, and up to which the sort's own blocks write
-// them.
+// Bytes of zeros from which the sort in one cluster hides behind the zeroing, and up to which the sort's own blocks
+// write them.
 constexpr int64_t kHidingBytes = 64 << 20;
 constexpr int64_t kSmallZeroBytes = 1 << 20;
 
@@ -194,9 +195,9 @@ int launch_grid_sort(GridSort& g, const ebr::keysort::Pass* pass, int passes, cu
   return EBR_OK;
 }
 
-// Sort n keys of [0, range]; digits: of one pass. For a route (route.row_of set) there is one pass, else the sorted keys
-// and positions are at *key / *order in the scratch. `zero_bytes` at `zero` (16-byte aligned) are zeroed beside or before
-// the sort.
+// Sort n keys of [0, range]; digits: of one pass. For a route (route.row_of set) there is one pass, else the sorted
+// keys and positions are at *key / *order in the scratch. `zero_bytes` at `zero` (16-byte aligned) are zeroed beside
+// or before the sort.
 int run_sort(int device, IdSource src, int64_t n, int passes, int bits, const ebr::keysort::RouteOut& route,
              void* scratch, int** key, int** order, void* zero, int64_t zero_bytes, cudaStream_t st) {
   char* at = static_cast<char*>(scratch);
@@ -276,8 +277,8 @@ int check_embedding(int id_type, int64_t n, int64_t V, int64_t C, int64_t stride
   return EBR_OK;
 }
 
-// Rows of a chunk of the gradient, 8 to 256: some 3,000 warps' worth of chunks (62,208 board tokens of 512 columns: the
-// whole gradient takes 35 us with 64 rows, 42 with 32, which leave twice the partial sums to join).
+// Rows of a chunk of the gradient, 8 to 256: some 3,000 warps' worth of chunks (62,208 board tokens of 512 columns:
+// the whole gradient takes 35 us with 64 rows, 42 with 32, which leave twice the partial sums to join).
 int64_t grad_chunk_rows(int64_t n, int64_t C) {
   const int64_t blocks = (C + 255) / 256;
   int64_t r = 8;
@@ -285,9 +286,9 @@ int64_t grad_chunk_rows(int64_t n, int64_t C) {
   return r;
 }
 
-// Gradients that one launch makes, the warps looking through all ids: few tokens, and as many warps as some waves of them. A
-// block owns a table row where the rows are few, up to kSomeTokens (500 tokens over ten ids: 4.2 us, 12.7 by way of the
-// sort), else a warp does, up to kFewTokens.
+// Gradients that one launch makes, the warps looking through all ids: few tokens, and as many warps as some waves of
+// them. A block owns a table row where the rows are few, up to kSomeTokens (500 tokens over ten ids: 4.2 us, 12.7 by
+// way of the sort), else a warp does, up to kFewTokens.
 constexpr int64_t kFewTokens = 128, kSomeTokens = 512;
 
 bool grad_by_blocks(int64_t n, int64_t V, int64_t C) { return n <= kSomeTokens && V * ((C + 255) / 256) <= 2048; }
@@ -300,9 +301,9 @@ bool grad_by_few(int64_t n, int64_t V, int64_t C) {
 constexpr int64_t kMaxVocabulary = int64_t{1} << 19;
 constexpr int kMaxEntries = 1024;
 
-// Rows of a few logits take four lanes each, rows of up to kWarpRowBytes a warp (half as much where there are not rows enough
-// to fill the GPU so), longer ones a ring of chunks. bfloat16, 2.1 GB of logits and gradient: a warp takes 0.52 ms at
-// V = 8,192 (the ring 0.72) and 0.57 at 16,384 (0.60).
+// Rows of a few logits take four lanes each, rows of up to kWarpRowBytes a warp (half as much where there are not
+// rows enough to fill the GPU so), longer ones a ring of chunks. bfloat16, 2.1 GB of logits and gradient: a warp
+// takes 0.52 ms at V = 8,192 (the ring 0.72) and 0.57 at 16,384 (0.60).
 constexpr int64_t kWarpRowBytes = 32 * 1024;
 
 bool distill_few(int64_t V, int64_t K) { return V <= 32 && K <= 32; }
@@ -344,8 +345,8 @@ int launch_distill_row(int device, const ebr::distill::Args& a, int slices, int 
   cfg.blockDim = dim3(kWarps * 32 + 32);
   cfg.dynamicSmemBytes = static_cast<size_t>(slots) * kWarps * kU * 512;
   const int64_t clusters = std::max<int64_t>(1, std::min<int64_t>(a.N, per_sm * sm_count(device) / slices));
-  // The rows' weights come from a kernel of their own (in `losses`, which the last kernel writes), unless no cluster has a
-  // second row: 12 rows of 151,665 float16 logits take 8.2 us without it, 9.5 with it.
+  // The rows' weights come from a kernel of their own (in `losses`, which the last kernel writes), unless no cluster
+  // has a second row: 12 rows of 151,665 float16 logits take 8.2 us without it, 9.5 with it.
   const float* weights = clusters < a.N ? a.losses : nullptr;
   if (weights) {
     ebr::distill::distill_weights_kernel<<<static_cast<unsigned>((a.N + 7) / 8), 256, 0, st>>>(a, a.losses);
@@ -388,9 +389,9 @@ int launch_distill(int device, const ebr::distill::Args& a, cudaStream_t st) {
   while (slices < ebr::distill::kMaxSlices && a.N * slices < 2 * sm_count(device) && (total + slices - 1) / slices > 256)
     slices *= 2;
   const int granules = static_cast<int>((total + slices - 1) / slices);
-  // Rows above 128 KB: rings of four 24 KB chunks, two on an SM, 24 warps; shorter rows want more rows in flight: rings of
-  // four 8 KB chunks, six on an SM. bfloat16 at 2.1 GB: V = 131,072 takes 0.44 ms with the first, 0.55 with the second;
-  // V = 32,768 takes 0.56 and 0.50.
+  // Rows above 128 KB: rings of four 24 KB chunks, two on an SM, 24 warps; shorter rows want more rows in flight:
+  // rings of four 8 KB chunks, six on an SM. bfloat16 at 2.1 GB: V = 131,072 takes 0.44 ms with the first, 0.55 with
+  // the second; V = 32,768 takes 0.56 and 0.50.
   const int rc = granules > 8192 ? launch_distill_row<T, 12, 4>(device, a, slices, granules, 4, 2, st)
                                  : launch_distill_row<T, 4, 4>(device, a, slices, granules, 4, 6, st);
   return rc != EBR_OK ? rc : launch_distill_entries<T, true>(a, st);
@@ -402,12 +403,16 @@ int launch_distill_grad(int device, const ebr::distill::Args& a, cudaStream_t st
   if (distill_by_warp<T>(a.N, a.V)) return launch_distill_warp<T, false>(a, st);
   constexpr int kThreads = 256;
   const int64_t total = row_granules<T>(a.V);
+  if (a.unless_one) {
+    ebr::distill::distill_grad_kernel<T, kThreads, true>
+        <<<static_cast<unsigned>(std::min<int64_t>(a.N, static_cast<int64_t>(sm_count(device)) * 4)), kThreads,
+           static_cast<size_t>(a.K) * 12, st>>>(a, 1, static_cast<int>(total));
+    return check_launch("topk_distill_grad");
+  }
   const int slices = static_cast<int>((total + 4095) / 4096);
-  const int64_t items = a.N * slices;
-  const int64_t most = static_cast<int64_t>(sm_count(device)) * (a.unless_one ? 8 : 64);
-  ebr::distill::distill_grad_kernel<T, kThreads>
-      <<<static_cast<unsigned>(std::min(items, most)), kThreads, 0, st>>>(
-          a, slices, static_cast<int>((total + slices - 1) / slices));
+  const int64_t blocks = std::min(a.N * slices, static_cast<int64_t>(sm_count(device)) * 64);
+  ebr::distill::distill_grad_kernel<T, kThreads, false><<<static_cast<unsigned>(blocks), kThreads, 0, st>>>(
+      a, slices, static_cast<int>((total + slices - 1) / slices));
   const int rc = check_launch("topk_distill_grad");
   return rc != EBR_OK ? rc : launch_distill_entries<T, false>(a, st);
 }
@@ -583,9 +588,9 @@ int ebr_scaled_embedding_grad(int g_dtype, int w_dtype, int id_type, int64_t n, 
 }  // extern "C"
 
 namespace {
-// Blocks along the tokens, each warp walking over several of them where there are many (board batch: dispatch 42 us with a
-// warp for each token, 38 so), and along the columns, where the tokens alone leave less than 96 warps to an SM (3,001
-// tokens of 999 float32, six rows each: cold, combine 54 us without, 29 with).
+// Blocks along the tokens, each warp walking over several of them where there are many (board batch: dispatch 42 us
+// with a warp for each token, 38 so), and along the columns, where the tokens alone leave less than 96 warps to an SM
+// (3,001 tokens of 999 float32, six rows each: cold, combine 54 us without, 29 with).
 dim3 expert_grid(int device, int64_t T, int64_t C, int per_trip, bool split) {
   const int64_t warps = int64_t{96} * sm_count(device);
   const int64_t parts = split ? std::max<int64_t>(1, std::min((C + per_trip - 1) / per_trip, warps / std::max<int64_t>(T, 1))) : 1;
