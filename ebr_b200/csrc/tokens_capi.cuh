@@ -696,7 +696,7 @@ int ebr_expert_combine(int dtype, int weight_dtype, int64_t T, int64_t K, int64_
     return set_error(EBR_ERR_SHAPE, "expert_combine: bad sizes%s%s");
   if (rows_stride < 0) return set_error(EBR_ERR_STRIDE, "expert_combine: negative stride%s%s");
   if (T == 0) return EBR_OK;
-  if (!row_of || !y) return set_error(EBR_ERR_NULL, "expert_combine: NULL pointer%s%s");
+  if (!rows_in || !row_of || !y) return set_error(EBR_ERR_NULL, "expert_combine: NULL pointer%s%s");
   int device = 0;
   if ((rc = check_device(&device)) != EBR_OK) return rc;
   auto st = static_cast<cudaStream_t>(stream);

@@ -57,7 +57,7 @@ int ebr_expert_scatter(int dtype, int weight_dtype, int64_t T, int64_t K, int64_
 
 /* And back: y[t, :] = round(sum over k of weights[t, k] * rows_in[row_of[t, k], :]) (weights NULL: ones), dropped slots
  * adding nothing (whatever their weights hold); rows_in [rows, C] (row stride rows_stride, unit column stride), y
- * [T, C] contiguous. Every row_of value is in [-1, rows). */
+ * [T, C] contiguous. There is at least one row, and every row_of value is in [-1, rows). */
 int ebr_expert_combine(int dtype, int weight_dtype, int64_t T, int64_t K, int64_t C, const void* rows_in,
                        int64_t rows_stride, const int32_t* row_of, const void* weights, void* y, void* stream);
 

@@ -78,7 +78,8 @@ def test_expert_refusals(lib):
     c = lambda **k: lib.ebr_expert_combine(*{**dict(d=BF16, w=F32, T=4, K=2, C=8, i=P, rs=8, r=P, wt=None, y=P, st=None),
                                              **k}.values())  # fmt: skip
     assert c(w=F16) == _native.ERR_DTYPE and c(T=-1) == _native.ERR_SHAPE and c(rs=-1) == _native.ERR_STRIDE
-    assert c(y=None) == _native.ERR_NULL and c(r=None) == _native.ERR_NULL and c(T=0, y=None, r=None) == _native.OK
+    assert c(y=None) == _native.ERR_NULL and c(r=None) == _native.ERR_NULL and c(i=None) == _native.ERR_NULL
+    assert c(T=0, y=None, r=None, i=None) == _native.OK
 
 
 def test_distillation_refusals(lib):
