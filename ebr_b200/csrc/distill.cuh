@@ -267,7 +267,8 @@ __global__ void __launch_bounds__(kSmallThreads) distill_small_kernel(const __gr
   if (any) {
     const float log_sum = logf(st.s);
     for (int k = lane; k < a.K; k += kLanes) {
-      const float d = p[k] - top, q = exp2_approx(d * a.exp2_scale) * inv_total;
+      // No entry, no probability: 0 times a total of NaN (a teacher's logit of NaN or infinity) is not 0.
+      const float d = p[k] - top, q = id[k] >= 0 ? exp2_approx(d * a.exp2_scale) * inv_total : 0.f;
       p[k] = q;
       if (kStats && (q > 0.f || isnan(q)))
         loss += q * ((d * a.inv_tau - log_total) - ((Elem<T>::load(row + id[k]) - st.m) * a.inv_tau - log_sum));
@@ -743,7 +744,8 @@ struct Entries {
   __device__ __forceinline__ float finish(const Args& a, const T* row, float m, float log_sum) {
     float loss = 0.f;
     for (int k = lane; k < a.K; k += 32) {
-      const float d = p[k] - top, q = exp2_approx(d * a.exp2_scale) * inv_total;
+      // No entry, no probability: 0 times a total of NaN (a teacher's logit of NaN or infinity) is not 0.
+      const float d = p[k] - top, q = id[k] >= 0 ? exp2_approx(d * a.exp2_scale) * inv_total : 0.f;
       p[k] = q;
       if (kLoss && (q > 0.f || isnan(q)))
         loss += q * ((d * a.inv_tau - log_total) - ((Elem<T>::load(row + id[k]) - m) * a.inv_tau - log_sum));

@@ -604,6 +604,43 @@ def test_distillation_of_a_masked_entry_and_non_finite_rows():
         assert g[1].isnan().all() and g[2].isnan().all() and g[3].isfinite().all()
 
 
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("n,v,k", [(70, 20, 5), (70, 10, 40), (300, 700, 5), (6, 40001, 5), (6, 40001, 70), (900, 33001, 5)])
+def test_distillation_of_a_non_finite_teacher_beside_padding(n, v, k, bad):
+    """A teacher's logit of NaN or infinity makes its own row's loss NaN, and the gradient of the logits that the row
+    names; padding entries of the same row name nothing and are read nowhere. Every kernel; the logits are an interior view."""
+    from ebr_b200.token_ops import topk_distill_loss
+
+    full = rand(n + 2, v + 16, seed=1, dtype=torch.bfloat16)
+    ids, good = randint(0, v, (n, k), seed=2), rand(n, k, seed=3)
+    hit = torch.zeros(n, dtype=torch.bool, device=DEV)
+    hit[[0, n // 2, n - 1]] = True
+    ids[:, 1] = -1
+    ids[hit, k // 2 :] = v + 3
+    top = good.clone()
+    top[hit, 0] = bad
+    top[:, 1] = bad  # of a padding entry: nothing
+    named = torch.zeros(n, v + 1, dtype=torch.bool, device=DEV)
+    named.scatter_(1, torch.where((ids >= 0) & (ids < v), ids, v), True)
+    named = named[:, :v] & hit.unsqueeze(1)
+    for how in ("none", "mean"):
+        results = []
+        for teacher in (good, top):
+            x = full[1:-1, 8 : v + 8].detach().requires_grad_(True)
+            loss = topk_distill_loss(x, ids, teacher, 1.5, reduction=how)
+            up = torch.ones_like(loss) if how == "none" else torch.tensor(0.5, device=DEV)
+            first = torch.autograd.grad(loss, x, torch.ones_like(loss), retain_graph=True)[0]
+            results.append((loss, first, torch.autograd.grad(loss, x, up)[0]))
+        (a, *ga), (b, *gb) = results
+        assert torch.equal(a[~hit], b[~hit]) and b[hit].isnan().all() if how == "none" else b.isnan()
+        for p, q in zip(ga, gb):
+            assert torch.equal(q.isnan(), named) and p.isfinite().all()
+            assert torch.equal(p[~named], q[~named])
+    with torch.no_grad():
+        rows = topk_distill_loss(full[1:-1, 8 : v + 8], ids, top, 1.5, reduction="none")
+    assert torch.equal(rows.isnan(), hit)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("v,wide", [(1000, 1024), (30001, 30016), (40001, 40960), (70003, 70005)])
 def test_distillation_of_strided_logits(v, wide, dtype):
