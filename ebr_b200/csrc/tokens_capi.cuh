@@ -172,12 +172,16 @@ int launch_zero(void* p, int64_t bytes, bool beside, cudaStream_t st) {
 }
 
 template <int kItems>
-int launch_grid_sort(GridSort& g, const ebr::keysort::Pass* pass, int passes, cudaStream_t st) {
+int launch_grid_sort(int device, GridSort& g, const ebr::keysort::Pass* pass, int passes, cudaStream_t st) {
   const size_t smem = ebr::keysort::grid_place_smem(g.digits);
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(ebr::keysort::grid_place_kernel<kItems>,
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  // The limit is the kernel's, not the call's: always the largest, so that no thread lowers it under another's launch.
+  static std::atomic<bool> ready[kMaxDevices];
+  if (device >= kMaxDevices || !ready[device].load()) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(ebr::keysort::grid_place_kernel<kItems>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(ebr::keysort::grid_place_smem(1 << ebr::keysort::kMaxDigitBits)));
     if (e != cudaSuccess) return cuda_error(e, "sort attributes");
+    if (device < kMaxDevices) ready[device].store(true);
   }
   g.scanned = g.tiles > ebr::keysort::kMaxTiles;
   for (int p = 0; p < passes; ++p) {
@@ -262,7 +266,8 @@ int run_sort(int device, IdSource src, int64_t n, int passes, int bits, const eb
   g.counts = take(static_cast<size_t>(g.digits) * g.tiles * 4);
   g.totals = take(static_cast<size_t>(g.digits) * 4);
   g.route = route;
-  return sort_items(n) == 2 ? launch_grid_sort<2>(g, pass, passes, st) : launch_grid_sort<8>(g, pass, passes, st);
+  return sort_items(n) == 2 ? launch_grid_sort<2>(device, g, pass, passes, st)
+                            : launch_grid_sort<8>(device, g, pass, passes, st);
 }
 
 // ------------------------------------------------------------------------------------------------ embedding

@@ -453,6 +453,34 @@ def test_expert_layer_replays_as_a_cuda_graph():
         assert torch.equal(out, layer())
 
 
+def test_expert_route_from_several_threads():
+    """Routes of different numbers of experts (of the sort's shared memory, that is) from threads of their own."""
+    import threading
+
+    from ebr_b200.token_ops import expert_route
+
+    failures = []
+
+    def work(experts):
+        try:
+            ids = randint(0, experts, (40000, 1), seed=experts)
+            with torch.cuda.stream(torch.cuda.Stream()):
+                first = expert_route(ids, experts)
+                for _ in range(6000):
+                    last = expert_route(ids, experts)
+                if not (torch.equal(first.row_of, last.row_of) and torch.equal(first.offsets, last.offsets)):
+                    failures.append(f"{experts} experts: another route")
+        except Exception as e:  # noqa: BLE001
+            failures.append(f"{experts} experts: {e}")
+
+    threads = [threading.Thread(target=work, args=(e,)) for e in (1024, 700, 1000, 800)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures, failures
+
+
 def test_expert_refusals():
     from ebr_b200.token_ops import expert_combine, expert_dispatch, expert_route
 
