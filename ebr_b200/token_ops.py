@@ -18,6 +18,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from ebr_b200 import _native
@@ -44,6 +45,23 @@ def _require(t: Tensor, what: str, name: str, types: dict, device: Optional[torc
         raise TypeError(f"{what}: unsupported dtype {t.dtype} of {name}")
     if device is not None and t.device != device:
         raise ValueError(f"{what}: {name} is on {t.device}, the other tensors are on {device}")
+
+
+def _has_tangent(*tensors: Optional[Tensor]) -> bool:
+    """Whether one of them carries a forward-mode tangent, which no kernel here propagates: such a call goes through its
+    autograd Function, which refuses it. A direct call would drop it, and a dropped tangent counts as zero."""
+    if forward_ad._current_level < 0:
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def _recorded(*tensors: Optional[Tensor]) -> bool:
+    """Whether a call goes through its autograd Function."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return _has_tangent(*tensors)
 
 
 def _fine(t: Tensor, types: dict) -> bool:
@@ -121,7 +139,7 @@ class _Embed(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g: Tensor):
         (tokens,) = ctx.saved_tensors
-        if torch.is_grad_enabled():
+        if torch.is_grad_enabled() or _has_tangent(g):
             return _EmbedGrad.apply(g, tokens, ctx.scale, ctx.rows, ctx.dtype), None, None, None
         return _lookup_grad(tokens, g, ctx.scale, ctx.rows, ctx.dtype), None, None, None
 
@@ -156,7 +174,7 @@ def scaled_embedding(tokens: Tensor, weight: Tensor, scale: float = 1.0, dtype: 
     if dtype not in _DTYPES:
         raise TypeError(f"scaled_embedding: unsupported output dtype {dtype}")
     tokens = tokens if tokens.is_contiguous() else tokens.contiguous()
-    if torch.is_grad_enabled() and weight.requires_grad:
+    if _recorded(weight):
         return _Embed.apply(weight, tokens, float(scale), dtype)
     return _lookup(tokens, weight, float(scale), dtype)
 
@@ -265,7 +283,7 @@ class _Dispatch(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g: Tensor):
         route = ctx.route
-        if not ctx.weighted and not torch.is_grad_enabled():
+        if not (ctx.weighted or torch.is_grad_enabled() or _has_tangent(g)):
             return _combine(g, route, None), None, None
         x, weights = ctx.saved_tensors if ctx.weighted else (None, None)
         gx = _Combine.apply(g, weights, route) if ctx.needs_input_grad[0] else None
@@ -289,7 +307,7 @@ class _Combine(torch.autograd.Function):
         route = ctx.route
         rows, weights = ctx.saved_tensors if ctx.weighted else (None, None)
         need_rows, need_weights = ctx.needs_input_grad[:2]
-        if need_rows and need_weights and ctx.weighted and not torch.is_grad_enabled():
+        if need_rows and need_weights and ctx.weighted and not torch.is_grad_enabled() and not _has_tangent(g):
             grows, gw = _scatter(_as(g, rows.dtype), route, weights, rows, True)  # both in one pass over g and the rows
             return grows, _as(gw, weights.dtype), None
         grows = _Dispatch.apply(g, weights, route) if need_rows else None
@@ -324,7 +342,7 @@ def expert_dispatch(x: Tensor, route: ExpertRoute) -> Tensor:
         raise ValueError(
             f"expert_dispatch: x must be [*{tuple(route.row_of.shape[:-1])}, C] for this route, got {tuple(x.shape)}"
         )
-    if torch.is_grad_enabled() and x.requires_grad:
+    if _recorded(x):
         return _Dispatch.apply(x, None, route)
     return _scatter(x, route, None, None, True)[0]
 
@@ -345,7 +363,7 @@ def expert_combine(rows: Tensor, route: ExpertRoute, weights: Optional[Tensor] =
             raise ValueError(
                 f"expert_combine: weights must be {tuple(route.row_of.shape)} for this route, got {tuple(weights.shape)}"
             )
-    if torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad)):
+    if _recorded(rows, weights):
         return _Combine.apply(rows, weights, route)
     return _combine(rows, route, weights)
 
@@ -431,6 +449,8 @@ class _TopkDistill(torch.autograd.Function):
 
     @staticmethod
     def _backward(ctx, g: Tensor):
+        if _has_tangent(g):
+            raise NotImplementedError("topk_distill_loss has no forward-mode derivative")
         logits, ids, top, row_weight, stats = ctx.saved_tensors
         made, ctx.made = ctx.made, None
         grad = _distill_gradient(logits, ids, top, ctx.tau, row_weight, ctx.factor, stats, g, made)
@@ -480,7 +500,7 @@ def topk_distill_loss(logits: Tensor, teacher_ids: Tensor, teacher_logits: Tenso
     rows = ids.numel() // ids.shape[-1]
     factor = 1.0 / rows if reduction == "mean" and rows else 1.0
     reduced = reduction != "none"
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if _recorded(logits, top, row_weight):
         return _TopkDistill.apply(logits, ids, top, float(temperature), row_weight, factor, reduced)
     losses, total, _, _ = _distill(logits, ids, top, float(temperature), row_weight, factor, reduced, False)
     return total if reduced else losses

@@ -766,6 +766,44 @@ def _plain_experts(net, blk, h):
     return out.view(h.shape)
 
 
+def test_forward_mode_is_refused():
+    """A forward-mode tangent of any input, or of an upstream gradient, is an error and not a derivative of zero."""
+    from torch.autograd import forward_ad
+
+    from ebr_b200.token_ops import expert_combine, expert_dispatch, expert_route, scaled_embedding, topk_distill_loss
+
+    tokens, w, x = randint(0, 6, (9,), seed=1), rand(6, 8, seed=2), rand(9, 8, seed=3)
+    r = expert_route(randint(0, 4, (9, 2), seed=4), 4)
+    rows, wt = rand(r.rows, 8, seed=5), rand(9, 2, seed=6)
+    ids, top, weight = randint(0, 8, (9, 3), seed=7), rand(9, 3, seed=8), rand(9, seed=9).abs()
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (
+            lambda: scaled_embedding(tokens, dual(w)),
+            lambda: expert_dispatch(dual(x), r),
+            lambda: expert_combine(dual(rows), r, wt),
+            lambda: expert_combine(rows, r, dual(wt)),
+            lambda: topk_distill_loss(dual(x), ids, top),
+            lambda: topk_distill_loss(x, ids, dual(top)),
+            lambda: topk_distill_loss(x, ids, top, row_weight=dual(weight), reduction="none"),
+        ):
+            with pytest.raises(NotImplementedError):
+                call()
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                call()
+        leaves = [t.clone().requires_grad_(True) for t in (w, x, rows, wt)]
+        ww, xx, rr, ll = leaves
+        for out, wrt in (
+            (scaled_embedding(tokens, ww), [ww]),
+            (expert_dispatch(xx, r), [xx]),
+            (expert_combine(rr, r, ll), [rr, ll]),
+            (topk_distill_loss(xx, ids, top, reduction="none"), [xx]),
+        ):
+            with pytest.raises(NotImplementedError):
+                torch.autograd.grad((out * dual(torch.ones_like(out))).sum(), wrt)
+        assert torch.equal(scaled_embedding(tokens, w), w[tokens])  # tensors without a tangent are as ever
+
+
 def test_expert_network_matches_plain_experts_to_second_order():
     """E, dE/dv and d<dE/dv, u>/d(v, weights) of the float32 network against the same network with a plain sparse MLP:
     1e-4 of the norms, the bar of the dense float32 network's fixtures."""
