@@ -6,9 +6,9 @@
 results back with the router's weights. Every step is differentiable to second order, as the descent's training needs it
 (dE/dz is itself differentiated), and nothing depends on the loads on the host, so microsteps replay as CUDA graphs.
 
-``distill_segment_loss`` trains either network on a teacher's top logits instead of labels: the board is embedded by
-``scaled_embedding``, the segment rolled out as in ``energy.train_segment_loss``, and the decoded endpoint's loss is
-``topk_distill_loss``. ``teacher_entries`` makes such entries from a trained network.
+``distill_segment_loss`` trains either network on a teacher's top logits instead of labels: the board is embedded as the
+network does it (``scaled_embedding`` here), the segment rolled out as in ``energy.train_segment_loss``, and the decoded
+endpoint's loss is ``topk_distill_loss``. ``teacher_entries`` makes such entries from a trained network.
 """
 
 from __future__ import annotations
@@ -101,7 +101,7 @@ def distill_segment_loss(net: LatentEnergyNet, z: Tensor, tokens: Tensor, teache
     ``graded`` with one, and the mean distillation loss of the decoded endpoint. ``cell_weight`` [B, L]: weights of the
     cells' losses (0 leaves a given cell out). Gradients reach the embedding through every graded microstep."""
     sigma = net.shape.noise_scale
-    x = scaled_embedding(tokens, net.embedding, math.sqrt(net.shape.hidden), net.shape.dtype)
+    x = net.embed(tokens)  # as in use: the dense network rounds its table before the product, the sparse one after
     with torch.no_grad():
         for _ in range(prefix):
             noise = torch.randn_like(z) * sigma if sigma else torch.zeros_like(z)

@@ -831,6 +831,24 @@ def test_expert_network_matches_plain_experts_to_second_order():
         assert float((a.double() - b.double()).norm()) <= 1e-4 * float(b.double().norm())
 
 
+@pytest.mark.parametrize("sparse", [False, True])
+def test_distillation_segment_embeds_as_the_network_does(sparse):
+    """The segment's input is the one that the network sees in use, bit for bit, and the embedding is trained through it."""
+    from ebr_b200.energy import LatentEnergyNet, NetShape
+    from ebr_b200.expert_net import ExpertEnergyNet, ExpertShape, distill_segment_loss
+
+    gen = torch.Generator().manual_seed(0)
+    net = ExpertEnergyNet(ExpertShape(layers=1), generator=gen) if sparse else LatentEnergyNet(NetShape(layers=1), generator=gen)
+    net = net.to(DEV)
+    tokens = randint(0, 10, (4, 81), seed=1)
+    ids, top = randint(0, 10, (4, 81, 3), seed=2), rand(4, 81, 3, seed=3)
+    seen, step = [], net.microstep
+    net.microstep = lambda z, x, **k: (seen.append(x.detach()), step(z, x, **k))[1]
+    distill_segment_loss(net, net.fresh_states(4), tokens, ids, top, prefix=0, graded=1).backward()
+    assert len(seen) == 1 and torch.equal(seen[0], net.embed(tokens))
+    assert net.embedding.grad.isfinite().all() and net.embedding.grad.any()
+
+
 def test_distillation_example_runs_and_learns():
     import importlib.util
     from pathlib import Path
