@@ -82,13 +82,29 @@ def _call(what: str, device: torch.device, fn, *args) -> None:
 
 
 def _row_view(t: Tensor) -> Tuple[Tensor, int]:
-    """(tensor, row stride) of ``t`` [..., C] seen as rows of C unit-stride elements; copies where it is not such a view."""
+    """(tensor, row stride) of ``t`` [..., C] seen as rows of C unit-stride elements; copies where no one stride leads
+    through all its rows."""
     c = t.shape[-1]
     if t.is_contiguous():
         return t, c
-    if t.dim() == 2 and (t.stride(1) == 1 or c == 1) and t.stride(0) >= 0:
-        return t, t.stride(0)
-    return t.contiguous(), c
+    stride = _row_stride(t)
+    return (t.contiguous(), c) if stride is None else (t, stride)
+
+
+def _row_stride(t: Tensor) -> Optional[int]:
+    """The stride between the rows of a tensor that is not contiguous, None where there is no single one."""
+    if t.stride(-1) != 1 and t.shape[-1] != 1:
+        return None
+    step, rows = None, 1  # the rows of the dimensions so far lie `step` apart
+    for size, stride in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if size == 1:
+            continue
+        if step is None:
+            step = stride
+        elif stride != step * rows:
+            return None
+        rows *= size
+    return t.shape[-1] if step is None else step
 
 
 def _scratch(nbytes: int, like: Tensor) -> Optional[Tensor]:
@@ -401,7 +417,7 @@ def _distill_gradient(logits: Tensor, ids: Tensor, top: Tensor, tau: float, row_
     if made is None:
         grad, grad_stride = _distill_grad_buffer(view, stride)
     else:
-        grad, grad_stride = made, _grad_stride(made)
+        grad, grad_stride = _row_view(made)
     if upstream.dtype != torch.float32:
         upstream = upstream.float()
     if upstream.dim() == 0 or not any(upstream.stride()):  # one value, or one value expanded over the rows
@@ -419,13 +435,13 @@ def _distill_grad_buffer(view: Tensor, stride: int) -> Tuple[Tensor, int]:
     """The gradient's buffer and row stride: contiguous, or with the logits' row stride where they are a view of slightly
     longer rows (a padded vocabulary), so that both rows start at the same place of a 16-byte word."""
     v = view.shape[-1]
-    if v < stride <= v + 256 and view.dim() == 2:
-        return torch.empty_strided(view.shape, view.stride(), device=view.device, dtype=view.dtype), stride
+    if v < stride <= v + 256 and view.dim() > 1:
+        strides, step = [1], stride
+        for size in reversed(view.shape[:-1]):
+            strides.append(step)
+            step *= size
+        return torch.empty_strided(view.shape, strides[::-1], device=view.device, dtype=view.dtype), stride
     return view.new_empty(view.shape), v
-
-
-def _grad_stride(grad: Tensor) -> int:
-    return grad.shape[-1] if grad.is_contiguous() else grad.stride(0)
 
 
 class _TopkDistill(torch.autograd.Function):

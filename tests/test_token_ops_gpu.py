@@ -688,6 +688,50 @@ def test_distillation_of_strided_logits(v, wide, dtype):
     check_distill(full[:, :v].reshape(1, 7, v), ids.view(1, 7, 9), top.view(1, 7, 9), 2.0)  # leading dimensions
 
 
+@pytest.mark.parametrize("v,wide", [(1001, 1024), (20001, 20016), (40001, 40960)])
+def test_distillation_of_a_padded_vocabulary_in_batches(v, wide):
+    """[B, L, :V] of [B, L, W]: the values, and no copy of the logits (the peak of the loss alone stays far below one)."""
+    from ebr_b200.token_ops import topk_distill_loss
+
+    full = (rand(3, 50, wide, seed=1) * 2).to(torch.bfloat16)
+    ids, top = randint(-1, v, (3, 50, 4), seed=2), rand(3, 50, 4, seed=3)
+    view = full[:, :, :v]
+    for logits in (view, view[:, ::2], view[1:2].transpose(0, 1), view[:, :1].expand(3, 50, v)):  # ... and strides that combine
+        i = ids[:, : logits.shape[1]] if logits.shape[0] == 3 else ids[1:2].transpose(0, 1)
+        t = top[:, : logits.shape[1]] if logits.shape[0] == 3 else top[1:2].transpose(0, 1)
+        check_distill(logits, i, t, 1.5)
+    x = view.detach().requires_grad_(True)
+    topk_distill_loss(x, ids, top, reduction="none")
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    held = torch.cuda.memory_allocated()
+    with torch.no_grad():
+        topk_distill_loss(x, ids, top, reduction="none")
+    assert torch.cuda.max_memory_allocated() - held < view.numel() // 2
+    loss = topk_distill_loss(x, ids, top)  # and its gradient, made in the forward pass
+    torch.autograd.grad(loss, x)
+    assert torch.cuda.max_memory_allocated() - held < 3 * full.numel()  # bytes: one gradient is two an element
+
+
+def test_rows_of_batched_views_are_read_in_place():
+    """Views whose leading dimensions share one row stride, and those that have none: the same values as their copies."""
+    from ebr_b200.token_ops import expert_combine, expert_dispatch, expert_route, scaled_embedding
+
+    big = rand(4, 6, 40, seed=1)
+    r = expert_route(randint(0, 5, (4, 6, 2), seed=2), 5)
+    w = rand(10, 34, seed=3).requires_grad_(True)
+    tokens = randint(0, 10, (4, 6), seed=4)
+    for view in (big[:, :, 3:37], big.transpose(0, 1)[:, :, :34].transpose(0, 1), rand(6, 4, 34, seed=5).transpose(0, 1),
+                 big[:1, :, :34].expand(4, 6, 34), big[:, :1, :34].expand(4, 6, 34), big[:1, :1, :34].expand(4, 6, 34),
+                 rand(34, 4, 6, seed=6).permute(1, 2, 0), rand(4, 6, 1, seed=7).expand(4, 6, 34)):  # fmt: skip
+        assert torch.equal(expert_dispatch(view, r), expert_dispatch(view.contiguous(), r))
+        x = torch.zeros(r.rows, 34, device=DEV, requires_grad=True)
+        a, b = (torch.autograd.grad(expert_combine(x, r), x, g)[0] for g in (view, view.contiguous()))
+        assert torch.equal(a, b)
+        a, b = (torch.autograd.grad(scaled_embedding(tokens, w), w, g)[0] for g in (view, view.contiguous()))
+        assert torch.equal(a, b)
+
+
 def test_distillation_repeats_bit_for_bit_on_other_streams_and_for_many_rows():
     from ebr_b200.token_ops import topk_distill_loss
 
