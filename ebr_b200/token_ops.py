@@ -393,27 +393,26 @@ def _distill_args(view: Tensor, ids: Tensor, top: Tensor, tau: float, factor: fl
     return (_DTYPES[view.dtype], _IDS[ids.dtype], _DTYPES[top.dtype], ids.numel() // k, view.shape[-1], k, tau, factor)
 
 
-def _distill(logits: Tensor, ids: Tensor, top: Tensor, tau: float, row_weight: Optional[Tensor], factor: float,
+def _distill(view: Tensor, stride: int, ids: Tensor, top: Tensor, tau: float, row_weight: Optional[Tensor], factor: float,
              total: bool, gradient: bool):  # fmt: skip
-    """(losses, total or None, stats, gradient or None): ``ebr_topk_distill``."""
-    view, stride = _row_view(logits)
+    """(losses, total or None, stats, gradient or None): ``ebr_topk_distill`` on a row view of the logits."""
     rows = ids.numel() // ids.shape[-1]
-    losses = logits.new_empty(ids.shape[:-1], dtype=torch.float32)
-    stats = logits.new_empty((rows, 2), dtype=torch.float32)
-    total = logits.new_empty((), dtype=torch.float32) if total else None
+    losses = view.new_empty(ids.shape[:-1], dtype=torch.float32)
+    stats = view.new_empty((rows, 2), dtype=torch.float32)
+    total = view.new_empty((), dtype=torch.float32) if total else None
     grad, grad_stride = _distill_grad_buffer(view, stride) if gradient else (None, 0)
-    _call("topk_distill_loss", logits.device, _native.lib().ebr_topk_distill,
+    _call("topk_distill_loss", view.device, _native.lib().ebr_topk_distill,
           *_distill_args(view, ids, top, tau, factor), view.data_ptr(), stride, ids.data_ptr(),
           top.data_ptr(), _ptr(row_weight), losses.data_ptr(), stats.data_ptr(), _ptr(total), _ptr(grad),
           grad_stride)  # fmt: skip
     return losses, total, stats, grad
 
 
-def _distill_gradient(logits: Tensor, ids: Tensor, top: Tensor, tau: float, row_weight: Optional[Tensor], factor: float,
+def _distill_gradient(view: Tensor, ids: Tensor, top: Tensor, tau: float, row_weight: Optional[Tensor], factor: float,
                       stats: Tensor, upstream: Tensor, made: Optional[Tensor]) -> Tensor:  # fmt: skip
-    """The gradient for ``upstream``, a scalar or one value per row: ``ebr_topk_distill_grad``. ``made``: the buffer that
-    the forward filled for an upstream of 1."""
-    view, stride = _row_view(logits)
+    """The gradient for ``upstream``, a scalar or one value per row: ``ebr_topk_distill_grad`` on the forward's row view.
+    ``made``: the buffer that the forward filled for an upstream of 1."""
+    view, stride = _row_view(view)
     if made is None:
         grad, grad_stride = _distill_grad_buffer(view, stride)
     else:
@@ -424,7 +423,7 @@ def _distill_gradient(logits: Tensor, ids: Tensor, top: Tensor, tau: float, row_
         per_row = 0
     else:
         upstream, per_row = upstream.contiguous(), 1
-    _call("topk_distill_loss", logits.device, _native.lib().ebr_topk_distill_grad,
+    _call("topk_distill_loss", view.device, _native.lib().ebr_topk_distill_grad,
           *_distill_args(view, ids, top, tau, factor), view.data_ptr(), stride, ids.data_ptr(),
           top.data_ptr(), _ptr(row_weight), stats.data_ptr(), upstream.data_ptr(), per_row, int(made is not None),
           grad.data_ptr(), grad_stride)  # fmt: skip
@@ -452,8 +451,9 @@ class _TopkDistill(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, ids, top, tau, row_weight, factor, reduced):
-        losses, total, stats, ctx.made = _distill(logits, ids, top, tau, row_weight, factor, reduced, reduced)
-        ctx.save_for_backward(logits, ids, top, row_weight, stats)
+        view, stride = _row_view(logits)  # saved as it is: a copy, where there has to be one, is made once
+        losses, total, stats, ctx.made = _distill(view, stride, ids, top, tau, row_weight, factor, reduced, reduced)
+        ctx.save_for_backward(view, ids, top, row_weight, stats)
         ctx.tau, ctx.factor = tau, factor
         return total if reduced else losses
 
@@ -467,9 +467,9 @@ class _TopkDistill(torch.autograd.Function):
     def _backward(ctx, g: Tensor):
         if _has_tangent(g):
             raise NotImplementedError("topk_distill_loss has no forward-mode derivative")
-        logits, ids, top, row_weight, stats = ctx.saved_tensors
+        view, ids, top, row_weight, stats = ctx.saved_tensors
         made, ctx.made = ctx.made, None
-        grad = _distill_gradient(logits, ids, top, ctx.tau, row_weight, ctx.factor, stats, g, made)
+        grad = _distill_gradient(view, ids, top, ctx.tau, row_weight, ctx.factor, stats, g, made)
         return grad, None, None, None, None, None, None
 
     _backward_once = staticmethod(once_differentiable(_backward.__func__))
@@ -485,7 +485,8 @@ def topk_distill_loss(logits: Tensor, teacher_ids: Tensor, teacher_logits: Tenso
     losses. A row without entries, or of weight 0, has loss 0 and gradient 0 whatever its logits hold. ``reduction``:
     ``"none"`` (the rows' losses, float32), ``"sum"`` or ``"mean"`` (the sum over the number of rows). Differentiable once,
     in ``logits``; the teacher and the weights are constants. A reduced loss keeps a gradient of the logits' size from the
-    forward to the backward pass."""
+    forward to the backward pass. Logits whose rows do not lie one stride apart are copied, once: leave positions out by
+    ``row_weight`` or padding ids rather than by a slice such as ``logits[:, :-1]``."""
     what = "topk_distill_loss"
     if not (_fine(logits, _DTYPES) and _fine(teacher_ids, _IDS) and _fine(teacher_logits, _DTYPES)
             and logits.device == teacher_ids.device == teacher_logits.device):  # fmt: skip
@@ -518,7 +519,7 @@ def topk_distill_loss(logits: Tensor, teacher_ids: Tensor, teacher_logits: Tenso
     reduced = reduction != "none"
     if _recorded(logits, top, row_weight):
         return _TopkDistill.apply(logits, ids, top, float(temperature), row_weight, factor, reduced)
-    losses, total, _, _ = _distill(logits, ids, top, float(temperature), row_weight, factor, reduced, False)
+    losses, total, _, _ = _distill(*_row_view(logits), ids, top, float(temperature), row_weight, factor, reduced, False)
     return total if reduced else losses
 
 

@@ -713,6 +713,27 @@ def test_distillation_of_a_padded_vocabulary_in_batches(v, wide):
     assert torch.cuda.max_memory_allocated() - held < 3 * full.numel()  # bytes: one gradient is two an element
 
 
+@pytest.mark.parametrize("how", ["none", "mean"])
+def test_distillation_copies_logits_without_a_row_stride_once(how):
+    """logits[:, :-1] of [B, L, V] has no one row stride: its copy is the forward's, and the backward makes none."""
+    from ebr_b200.token_ops import topk_distill_loss
+
+    full = rand(3, 51, 20000, seed=1, dtype=torch.bfloat16)
+    view = full[:, :-1]
+    ids, top = randint(-1, 20000, (3, 50, 4), seed=2), rand(3, 50, 4, seed=3)
+    check_distill(view, ids, top, 1.5)
+    for up in (1.0, 2.0):
+        x = view.detach().requires_grad_(True)
+        loss = topk_distill_loss(x, ids, top, reduction=how)
+        upstream = torch.full_like(loss, up)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        held = torch.cuda.memory_allocated()
+        torch.autograd.grad(loss, x, upstream)
+        gradient = 2 * view.numel() if how == "none" else 0  # bytes; a reduced loss holds it already
+        assert torch.cuda.max_memory_allocated() - held <= gradient + (1 << 20)
+
+
 def test_rows_of_batched_views_are_read_in_place():
     """Views whose leading dimensions share one row stride, and those that have none: the same values as their copies."""
     from ebr_b200.token_ops import expert_combine, expert_dispatch, expert_route, scaled_embedding
