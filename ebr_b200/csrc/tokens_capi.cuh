@@ -305,6 +305,7 @@ bool grad_by_few(int64_t n, int64_t V, int64_t C) {
 
 constexpr int64_t kMaxVocabulary = int64_t{1} << 19;
 constexpr int kMaxEntries = 1024;
+constexpr double kLeastTau = 0x1p-126;  // the smallest normal float: log2(e) / tau is finite
 
 // Rows of a few logits take four lanes each, rows of up to kWarpRowBytes a warp (half as much where there are not
 // rows enough to fill the GPU so), longer ones a ring of chunks. bfloat16, 2.1 GB of logits and gradient: a warp
@@ -430,7 +431,8 @@ int check_distill(int dtype, int id_type, int top_dtype, int64_t N, int64_t V, i
   if (rc != EBR_OK) return rc;
   if (N < 0 || V < 1 || K < 1 || K > kMaxEntries) return set_error(EBR_ERR_SHAPE, "topk_distill: bad sizes%s%s");
   if (N >= (int64_t{1} << 31) || V > kMaxVocabulary) return set_error(EBR_ERR_SHAPE, "topk_distill: size too large%s%s");
-  if (!(tau > 0.0) || tau > 1e30) return set_error(EBR_ERR_SHAPE, "topk_distill: the temperature must be positive%s%s");
+  if (!(tau >= kLeastTau && tau <= 1e30))
+    return set_error(EBR_ERR_SHAPE, "topk_distill: the temperature must be between 1.2e-38 and 1e30%s%s");
   if (stride < 0 || grad_stride < V) return set_error(EBR_ERR_STRIDE, "topk_distill: bad row stride%s%s");
   return EBR_OK;
 }
@@ -443,7 +445,6 @@ ebr::distill::Args distill_args(int64_t N, int64_t V, int64_t K, double tau, dou
   a.V = V;
   a.K = static_cast<int>(K);
   a.tau = static_cast<float>(tau);
-  a.inv_tau = static_cast<float>(1.0 / tau);
   a.exp2_scale = static_cast<float>(1.4426950408889634 / tau);
   a.factor = static_cast<float>(factor);
   a.logits = logits;

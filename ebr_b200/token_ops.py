@@ -501,8 +501,8 @@ def topk_distill_loss(logits: Tensor, teacher_ids: Tensor, teacher_logits: Tenso
                          f"{tuple(teacher_logits.shape)} and {tuple(teacher_ids.shape)}")  # fmt: skip
     if logits.shape[-1] > 1 << 19:
         raise ValueError(f"{what}: a vocabulary of at most {1 << 19}, got {logits.shape[-1]}")
-    if not temperature > 0:
-        raise ValueError(f"{what}: the temperature must be positive, got {temperature}")
+    if not 2.0**-126 <= temperature <= 1e30:
+        raise ValueError(f"{what}: the temperature must be between 1.2e-38 and 1e30, got {temperature}")
     if reduction not in ("none", "sum", "mean"):
         raise ValueError(f"{what}: reduction must be 'none', 'sum' or 'mean', got {reduction!r}")
     if teacher_logits.requires_grad or (row_weight is not None and row_weight.requires_grad):

@@ -103,6 +103,14 @@ def test_distillation_refusals(lib):
     assert g(N=0, x=None) == _native.OK
 
 
+def test_distillation_temperatures(lib):
+    args = lambda tau, x: (BF16, 1, F32, 4, 100, 3, tau, 1.0, x, 100, P, P, None, P, P, None, None, 0, None)  # noqa: E731
+    for bad in (0.0, -1.0, 1e-39, 1.1e30, float("inf"), float("nan")):
+        assert lib.ebr_topk_distill(*args(bad, None)) == _native.ERR_SHAPE, bad
+    for good in (2.0**-126, 1.0, 1e30):
+        assert lib.ebr_topk_distill(*args(good, None)) == _native.ERR_NULL, good  # accepted; the logits are missing
+
+
 def test_python_operators_refuse_cpu_tensors():
     from ebr_b200 import token_ops as tk
 

@@ -615,6 +615,45 @@ def test_distillation_masks(v):
         check_distill(x, i, t, 1.3, weight)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tau,share", [(1e-37, 1.0), (1e-30, 1.0), (1e-12, 1.0), (2.5e19, 0.01), (1e21, 1e-6)])
+@pytest.mark.parametrize("n,v,k", [(4, 10, 9), (4, 700, 60), (4, 40001, 900)])
+def test_distillation_at_extreme_temperatures(n, v, k, tau, share, dtype):
+    """Losses that float32 holds, at temperatures whose square or inverse it does not. Beside the tolerances above, the
+    rounding of the temperature and of the products with it and with the weight: 16 e of the loss, 8 e of the gradient."""
+    from ebr_b200.token_ops import topk_distill_loss
+
+    logits, ids, top = (rand(n, v, seed=1) * 3).to(dtype), randint(0, v, (n, k), seed=2), rand(n, k, seed=3)
+    weight = torch.full((n,), share, device=DEV)
+    ref, grad, q, mass, largest = plain_distill(logits, ids, top, tau, weight)
+    assert float(ref.abs().max()) < 3e38
+    r = relative(v)
+    x = logits.clone().requires_grad_(True)
+    rows = topk_distill_loss(x, ids, top, tau, row_weight=weight, reduction="none")
+    assert_within(rows, ref, share * tau**2 * (2 * r + 4 * E * (1 + largest)) + 16 * E * ref.abs() + 1e-44)
+    bound = share * tau * (2 * r + 4 * E) * (q + mass) + (U[dtype] + 8 * E) * grad.abs() + 1e-38
+    assert_within(torch.autograd.grad(rows, x, torch.ones_like(rows))[0], grad, bound)
+    total = topk_distill_loss(x, ids, top, tau, row_weight=weight)
+    assert_within(torch.autograd.grad(total, x)[0], grad / n, bound / n + 1e-38)
+
+
+def test_distillation_of_an_entry_at_the_lowest_value():
+    """A masked logit that the teacher names: tau p 3.4e38, which float32 holds at tau = 0.5."""
+    from ebr_b200.token_ops import topk_distill_loss
+
+    for dtype in (torch.float32, torch.bfloat16):
+        for v in (12, 600, 40000):
+            x = rand(3, v, seed=1).to(dtype)
+            x[1, 5] = torch.finfo(dtype).min
+            x.requires_grad_(True)
+            ids, top = torch.tensor([[5, 6]] * 3, device=DEV), torch.zeros(3, 2, device=DEV)
+            ref, grad, *_ = plain_distill(x.detach(), ids, top, 0.5)
+            rows = topk_distill_loss(x, ids, top, 0.5, reduction="none")
+            assert float(ref[1]) > 8e37 and abs(float(rows.detach()[1]) / float(ref[1]) - 1) < 1e-5
+            (g,) = torch.autograd.grad(rows, x, torch.ones_like(rows))
+            assert float((g.double() - grad).abs().max()) <= 2 * U[dtype] + 1e-5
+
+
 def test_distillation_of_a_masked_entry_and_non_finite_rows():
     from ebr_b200.token_ops import topk_distill_loss
 
