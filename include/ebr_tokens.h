@@ -68,8 +68,8 @@ int ebr_expert_combine(int dtype, int weight_dtype, int64_t T, int64_t K, int64_
  *   losses[n] = w_n * tau^2 * sum over the entries of p_k (log p_k - log q[id_k]),
  *   total = factor * sum over n of losses[n],
  *   grad[n, j] = factor * u_n * w_n * tau * (q_j - sum of p_k with id_k = j),
- * entries with p_k = 0 adding nothing. A row without entries, or with w_n = 0, has loss 0 and gradient 0 whatever its
- * logits hold. 1 <= K <= 1024, 1 <= V <= 2^19, 2^-126 <= tau <= 1e30.
+ * entries with p_k = 0 adding nothing. A row without entries, or with entries of -infinity alone (a teacher's mask that
+ * leaves nothing), or with w_n = 0, has loss 0 and gradient 0 whatever its logits hold. 1 <= K <= 1024, 1 <= V <= 2^19, 2^-126 <= tau <= 1e30.
  *
  * ebr_topk_distill: losses [N] float32; stats [N, 2] float32, 8-byte aligned (each row's largest logit and its sum of
  * exp((s - largest) / tau); 0 and infinity for a row that does not count); total: one float32 (a sum in a fixed order), or NULL; grad [N, V] of type dtype

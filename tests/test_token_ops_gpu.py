@@ -637,6 +637,16 @@ def test_distillation_at_extreme_temperatures(n, v, k, tau, share, dtype):
     assert_within(torch.autograd.grad(total, x)[0], grad / n, bound / n + 1e-38)
 
 
+@pytest.mark.parametrize("n,v", [(9, 10), (9, 700), (9, 40001), (900, 33001)])
+def test_distillation_of_a_teacher_that_is_masked_out(n, v):
+    """Entries of -inf alone are no entries: loss 0 and gradient 0, even of NaN logits; the other rows do not notice."""
+    x, ids, top = rand(n, v, seed=1), randint(0, v, (n, 3), seed=2), rand(n, 3, seed=3)
+    top[[0, 4, 5, n - 1]] = -math.inf
+    ids[5, 1] = -1
+    x[4] = math.nan
+    check_distill(x.to(torch.bfloat16), ids, top, 1.4)
+
+
 def test_distillation_of_an_entry_at_the_lowest_value():
     """A masked logit that the teacher names: tau p 3.4e38, which float32 holds at tau = 0.5."""
     from ebr_b200.token_ops import topk_distill_loss
