@@ -45,6 +45,23 @@ class ExpertShape(NetShape):
         return max(1, math.ceil(self.capacity_factor * cells * self.experts_per_cell / self.experts))
 
 
+class _RouterScores(torch.autograd.Function):
+    """h W^T in float32, h and W as they are: scores rounded to 16 bits would leave near ties between experts to the
+    rounding. The backward is a 16-bit product's, with the scores' gradient rounded as any activation's, and is
+    differentiable. (Casting h and W to float32 instead took a training step of 768 boards from 24 to 26 ms.)"""
+
+    @staticmethod
+    def forward(ctx, h: Tensor, w: Tensor) -> Tensor:
+        ctx.save_for_backward(h, w)
+        return torch.mm(h, w.t()) if h.dtype == torch.float32 else torch.mm(h, w.t(), out_dtype=torch.float32)
+
+    @staticmethod
+    def backward(ctx, g: Tensor):
+        h, w = ctx.saved_tensors
+        g = g.to(h.dtype)
+        return g @ w, g.t() @ h
+
+
 class ExpertEnergyNet(LatentEnergyNet):
     def __init__(self, shape: ExpertShape, attention: Optional[AttentionFn] = None,
                  generator: Optional[torch.Generator] = None) -> None:  # fmt: skip
@@ -66,7 +83,7 @@ class ExpertEnergyNet(LatentEnergyNet):
 
     def _experts(self, blk: nn.Module, h: Tensor) -> Tensor:
         s, dt, c = self.shape, h.dtype, h.shape[-1]
-        scores = F.linear(h, blk.router.to(dt)).float()
+        scores = _RouterScores.apply(h.reshape(-1, c), blk.router.to(dt)).view(*h.shape[:-1], s.experts)
         best, ids = scores.topk(s.experts_per_cell, dim=-1)
         route = expert_route(ids, s.experts, s.capacity(h.numel() // c))
         rows = expert_dispatch(h, route).view(s.experts, -1, c)

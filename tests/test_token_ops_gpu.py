@@ -945,6 +945,28 @@ def test_expert_network_matches_plain_experts_to_second_order():
         assert float((a.double() - b.double()).norm()) <= 1e-4 * float(b.double().norm())
 
 
+def test_expert_network_routes_by_float32_scores(monkeypatch):
+    """The bfloat16 network's choices are those of the float64 product of its activations with the bfloat16 router, wherever
+    the scores of the chosen and of the others differ by more than the float32 product's rounding."""
+    from ebr_b200 import expert_net
+    from ebr_b200.expert_net import ExpertEnergyNet, ExpertShape
+
+    net = ExpertEnergyNet(ExpertShape(layers=1), generator=torch.Generator().manual_seed(0)).to(DEV)
+    seen, route = [], expert_net.expert_route
+    monkeypatch.setattr(expert_net, "expert_route", lambda ids, *a: (seen.append(ids), route(ids, *a))[1])
+    h = rand(40, 81, 512, seed=1, dtype=torch.bfloat16)
+    router = net.blocks[0].router.detach().bfloat16()
+    with torch.no_grad():
+        out = net._experts(net.blocks[0], h)
+    assert out.dtype == torch.bfloat16
+    exact = h.double() @ router.double().t()
+    magnitude = h.double().abs() @ router.double().abs().t()
+    best, ids = exact.topk(net.shape.experts_per_cell + 1, dim=-1)
+    clear = ((best[..., :-1] - best[..., 1:]) > 2 * 514 * E * magnitude.max(-1, keepdim=True).values).all(-1)
+    assert float(clear.double().mean()) > 0.95
+    assert torch.equal(seen[0][clear], ids[..., :-1][clear])
+
+
 @pytest.mark.parametrize("sparse", [False, True])
 def test_distillation_segment_embeds_as_the_network_does(sparse):
     """The segment's input is the one that the network sees in use, bit for bit, and the embedding is trained through it."""
