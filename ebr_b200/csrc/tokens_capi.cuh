@@ -305,6 +305,8 @@ bool grad_by_few(int64_t n, int64_t V, int64_t C) {
 
 constexpr int64_t kMaxVocabulary = int64_t{1} << 19;
 constexpr int kMaxEntries = 1024;
+// The long rows' kernel counts rows in an int, in steps of up to six clusters for each SM: the last step has to fit, too.
+constexpr int64_t kMaxRows = (int64_t{1} << 31) - (1 << 16);
 constexpr double kLeastTau = 0x1p-126;  // the smallest normal float: log2(e) / tau is finite
 
 // Rows of a few logits take four lanes each, rows of up to kWarpRowBytes a warp (half as much where there are not
@@ -430,7 +432,7 @@ int check_distill(int dtype, int id_type, int top_dtype, int64_t N, int64_t V, i
   if (rc == EBR_OK) rc = check_id_type(id_type);
   if (rc != EBR_OK) return rc;
   if (N < 0 || V < 1 || K < 1 || K > kMaxEntries) return set_error(EBR_ERR_SHAPE, "topk_distill: bad sizes%s%s");
-  if (N >= (int64_t{1} << 31) || V > kMaxVocabulary) return set_error(EBR_ERR_SHAPE, "topk_distill: size too large%s%s");
+  if (N >= kMaxRows || V > kMaxVocabulary) return set_error(EBR_ERR_SHAPE, "topk_distill: size too large%s%s");
   if (!(tau >= kLeastTau && tau <= 1e30))
     return set_error(EBR_ERR_SHAPE, "topk_distill: the temperature must be between 1.2e-38 and 1e30%s%s");
   if (stride < 0 || grad_stride < V) return set_error(EBR_ERR_STRIDE, "topk_distill: bad row stride%s%s");

@@ -69,11 +69,12 @@ int ebr_expert_combine(int dtype, int weight_dtype, int64_t T, int64_t K, int64_
  *   total = factor * sum over n of losses[n],
  *   grad[n, j] = factor * u_n * w_n * tau * (q_j - sum of p_k with id_k = j),
  * entries with p_k = 0 adding nothing. A row without entries, or with entries of -infinity alone (a teacher's mask that
- * leaves nothing), or with w_n = 0, has loss 0 and gradient 0 whatever its logits hold. 1 <= K <= 1024, 1 <= V <= 2^19, 2^-126 <= tau <= 1e30.
+ * leaves nothing), or with w_n = 0, has loss 0 and gradient 0 whatever its logits hold. 1 <= K <= 1024, 1 <= V <= 2^19,
+ * N < 2^31 - 2^16, 2^-126 <= tau <= 1e30.
  *
  * ebr_topk_distill: losses [N] float32; stats [N, 2] float32, 8-byte aligned (each row's largest logit and its sum of
- * exp((s - largest) / tau); 0 and infinity for a row that does not count); total: one float32 (a sum in a fixed order), or NULL; grad [N, V] of type dtype
- * (row stride grad_stride, unit column stride), made with u_n = 1, or NULL.
+ * exp((s - largest) / tau); 0 and infinity for a row that does not count); total: one float32 (a sum in a fixed order),
+ * or NULL; grad [N, V] of type dtype (row stride grad_stride, unit column stride), made with u_n = 1, or NULL.
  * ebr_topk_distill_grad: grad from the forward's stats, u_n = upstream[upstream_stride * n] (stride 0 or 1). With
  * unless_one != 0 and stride 0, nothing is written where upstream[0] is exactly 1: grad was made with it already. */
 int ebr_topk_distill(int dtype, int id_type, int top_dtype, int64_t N, int64_t V, int64_t K, double tau, double factor,

@@ -111,6 +111,14 @@ def test_distillation_temperatures(lib):
         assert lib.ebr_topk_distill(*args(good, None)) == _native.ERR_NULL, good  # accepted; the logits are missing
 
 
+def test_distillation_rows(lib):
+    """The number of rows leaves room for the last step of a kernel's row counter, an int."""
+    args = lambda n: (BF16, 1, F32, n, 100, 3, 1.0, 1.0, None, 100, P, P, None, P, P, None, None, 0, None)  # noqa: E731
+    for n in ((1 << 31) - 1, (1 << 31) - 148 * 6, (1 << 31) - (1 << 16)):
+        assert lib.ebr_topk_distill(*args(n)) == _native.ERR_SHAPE, n
+    assert lib.ebr_topk_distill(*args((1 << 31) - (1 << 16) - 1)) == _native.ERR_NULL  # accepted; the logits are missing
+
+
 def test_python_operators_refuse_cpu_tensors():
     from ebr_b200 import token_ops as tk
 
