@@ -29,6 +29,18 @@ int check_ids(const void* ids, int id_type) {
   return on_boundary(ids, id_type == EBR_INT64 ? 8 : 4) ? EBR_OK : set_error(EBR_ERR_STRIDE, "unaligned ids%s%s");
 }
 
+// Arrays that start where none of their elements may are refused here: in a kernel they would be a fault.
+struct Array {
+  const void* p;
+  size_t size;
+};
+
+int check_arrays(std::initializer_list<Array> arrays) {
+  for (const Array& a : arrays)
+    if (!on_boundary(a.p, a.size)) return set_error(EBR_ERR_STRIDE, "an array is not aligned to its elements%s%s");
+  return EBR_OK;
+}
+
 size_t round16(size_t b) { return (b + 15) & ~size_t{15}; }
 
 // Run fn(tag of A, tag of B) for two I/O types.
@@ -472,6 +484,7 @@ int ebr_scaled_embedding(int w_dtype, int out_dtype, int id_type, int64_t n, int
   if (n == 0) return EBR_OK;
   if (!ids || !w || !out) return set_error(EBR_ERR_NULL, "scaled_embedding: NULL pointer%s%s");
   if ((rc = check_ids(ids, id_type)) != EBR_OK) return rc;
+  if ((rc = check_arrays({{w, elem_size(w_dtype)}, {out, elem_size(out_dtype)}})) != EBR_OK) return rc;
   int device = 0;
   if ((rc = check_device(&device)) != EBR_OK) return rc;
   auto st = static_cast<cudaStream_t>(stream);
@@ -526,6 +539,7 @@ int ebr_scaled_embedding_grad(int g_dtype, int w_dtype, int id_type, int64_t n, 
   }
   if (!ids || !g) return set_error(EBR_ERR_NULL, "scaled_embedding_grad: NULL pointer%s%s");
   if ((rc = check_ids(ids, id_type)) != EBR_OK) return rc;
+  if ((rc = check_arrays({{g, elem_size(g_dtype)}})) != EBR_OK) return rc;
   if (!aligned16(dw)) return set_error(EBR_ERR_STRIDE, "scaled_embedding_grad: dW must be 16-byte aligned%s%s");
   const size_t need = ebr_scaled_embedding_grad_scratch_bytes(n, V, C);
   if (need && (!scratch || !aligned16(scratch) || scratch_bytes < need))
@@ -626,6 +640,7 @@ int ebr_expert_route(int id_type, int64_t T, int64_t K, int64_t E, int64_t capac
   const int64_t n = T * K, rows = capacity ? E * capacity : n;
   if (!offsets || (n && (!ids || !row_of)) || (rows && !slot_of)) return set_error(EBR_ERR_NULL, "expert_route: NULL pointer%s%s");
   if ((rc = check_ids(ids, id_type)) != EBR_OK) return rc;
+  if ((rc = check_arrays({{row_of, 4}, {slot_of, 4}, {offsets, 4}})) != EBR_OK) return rc;
   const size_t need = ebr_expert_route_scratch_bytes(T, K, E);
   if (need && (!scratch || !aligned16(scratch) || scratch_bytes < need))
     return set_error(EBR_ERR_SCRATCH, "expert_route: scratch too small or unaligned%s%s");
@@ -660,6 +675,10 @@ int ebr_expert_scatter(int dtype, int weight_dtype, int64_t T, int64_t K, int64_
     return set_error(EBR_ERR_NULL, "expert_scatter: rows_in and dots go together%s%s");
   if ((T && (!x || !row_of)) || (rows && rows_out && !slot_of)) return set_error(EBR_ERR_NULL, "expert_scatter: NULL pointer%s%s");
   if (T == 0 && (rows == 0 || !rows_out)) return EBR_OK;
+  const size_t size_x = elem_size(dtype), size_w = elem_size(weight_dtype);
+  rc = check_arrays({{x, size_x}, {rows_in, size_x}, {rows_out, size_x}, {row_of, 4}, {slot_of, 4}, {weights, size_w},
+                     {dots, size_w}});
+  if (rc != EBR_OK) return rc;
   int device = 0;
   if ((rc = check_device(&device)) != EBR_OK) return rc;
   auto st = static_cast<cudaStream_t>(stream);
@@ -705,6 +724,9 @@ int ebr_expert_combine(int dtype, int weight_dtype, int64_t T, int64_t K, int64_
   if (rows_stride < 0) return set_error(EBR_ERR_STRIDE, "expert_combine: negative stride%s%s");
   if (T == 0) return EBR_OK;
   if (!rows_in || !row_of || !y) return set_error(EBR_ERR_NULL, "expert_combine: NULL pointer%s%s");
+  const size_t size_x = elem_size(dtype);
+  if ((rc = check_arrays({{rows_in, size_x}, {y, size_x}, {row_of, 4}, {weights, elem_size(weight_dtype)}})) != EBR_OK)
+    return rc;
   int device = 0;
   if ((rc = check_device(&device)) != EBR_OK) return rc;
   auto st = static_cast<cudaStream_t>(stream);
@@ -741,6 +763,9 @@ int ebr_topk_distill(int dtype, int id_type, int top_dtype, int64_t N, int64_t V
   if (N && (!logits || !top_ids || !top_logits || !losses || !stats)) return set_error(EBR_ERR_NULL, "topk_distill: NULL pointer%s%s");
   if ((rc = check_ids(top_ids, id_type)) != EBR_OK) return rc;
   if (!on_boundary(stats, 8)) return set_error(EBR_ERR_STRIDE, "topk_distill: unaligned stats%s%s");
+  rc = check_arrays({{logits, elem_size(dtype)}, {top_logits, elem_size(top_dtype)}, {row_weight, 4}, {losses, 4},
+                     {total, 4}, {grad, elem_size(dtype)}});
+  if (rc != EBR_OK) return rc;
   int device = 0;
   if ((rc = check_device(&device)) != EBR_OK) return rc;
   auto st = static_cast<cudaStream_t>(stream);
@@ -775,6 +800,9 @@ int ebr_topk_distill_grad(int dtype, int id_type, int top_dtype, int64_t N, int6
     return set_error(EBR_ERR_NULL, "topk_distill_grad: NULL pointer%s%s");
   if ((rc = check_ids(top_ids, id_type)) != EBR_OK) return rc;
   if (!on_boundary(stats, 8)) return set_error(EBR_ERR_STRIDE, "topk_distill_grad: unaligned stats%s%s");
+  rc = check_arrays({{logits, elem_size(dtype)}, {top_logits, elem_size(top_dtype)}, {row_weight, 4}, {upstream, 4},
+                     {grad, elem_size(dtype)}});
+  if (rc != EBR_OK) return rc;
   int device = 0;
   if ((rc = check_device(&device)) != EBR_OK) return rc;
   ebr::distill::Args a = distill_args(N, V, K, tau, factor, id_type, top_dtype, logits, logits_stride, top_ids,

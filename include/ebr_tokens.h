@@ -5,7 +5,8 @@
  * nothing allocated, nothing trapped, no host synchronisation. Every function returns EBR_OK (0) or an ebr_status code;
  * ebr_attn_last_error() holds the message. I/O types are EBR_FLOAT32 / EBR_FLOAT16 / EBR_BFLOAT16; sums, softmax
  * statistics and losses are float32 in a fixed order (the same inputs give the same bits), with one rounding to the
- * output's type. Scratch buffers are 16-byte aligned, of at least the bytes that the *_scratch_bytes function gives.
+ * output's type. Scratch buffers are 16-byte aligned, of at least the bytes that the *_scratch_bytes function gives;
+ * other arrays start at a multiple of their elements' size, unless more is said, else EBR_ERR_STRIDE.
  */
 #ifndef EBR_TOKENS_H
 #define EBR_TOKENS_H

@@ -119,6 +119,30 @@ def test_distillation_rows(lib):
     assert lib.ebr_topk_distill(*args((1 << 31) - (1 << 16) - 1)) == _native.ERR_NULL  # accepted; the logits are missing
 
 
+def test_arrays_that_start_inside_an_element_are_refused(lib):
+    """A 16-bit array at an odd address and a 32-bit one at an address of 2 mod 4, in every place that takes one."""
+    one = dict(n=4, V=10, C=8)
+    lookup = dict(w=F32, o=BF16, i=1, **one, s=1.0, ids=P, p=P, ws=8, out=P, st=None)
+    grad = dict(g=BF16, w=F32, i=1, **one, s=1.0, ids=P, p=P, gs=8, dw=P, sc=None, b=0, st=None)
+    route = dict(i=0, T=4, K=2, E=8, c=0, ids=P, r=P, s=P, o=P, sc=None, b=0, st=None)
+    scatter = dict(d=BF16, w=F32, T=4, K=2, C=8, R=8, x=P, xs=8, r=P, s=P, wt=P, i=P, o=P, dots=P, st=None)
+    combine = dict(d=BF16, w=F32, T=4, K=2, C=8, i=P, rs=8, r=P, wt=P, y=P, st=None)
+    sizes = dict(N=4, V=100, K=3, tau=1.0, f=1.0)
+    distill = dict(d=BF16, i=1, t=F32, **sizes, x=P, xs=100, ids=P, top=P, rw=P, l=P, s=P, tot=P, g=P, gs=100, st=None)
+    back = dict(d=BF16, i=1, t=F32, **sizes, x=P, xs=100, ids=P, top=P, rw=P, s=P, u=P, us=0, one=0, g=P, gs=100, st=None)
+    for name, args, halves, words in (
+        ("ebr_scaled_embedding", lookup, ("out",), ("p",)),
+        ("ebr_scaled_embedding_grad", grad, ("p",), ("dw",)),
+        ("ebr_expert_route", route, (), ("ids", "r", "s", "o")),
+        ("ebr_expert_scatter", scatter, ("x", "i", "o"), ("r", "s", "wt", "dots")),
+        ("ebr_expert_combine", combine, ("i", "y"), ("r", "wt")),
+        ("ebr_topk_distill", distill, ("x", "g"), ("ids", "top", "rw", "l", "s", "tot")),
+        ("ebr_topk_distill_grad", back, ("x", "g"), ("ids", "top", "rw", "s", "u")),
+    ):
+        for place, off in [(a, 1) for a in halves] + [(a, 2) for a in words]:
+            assert getattr(lib, name)(*{**args, place: P + off}.values()) == _native.ERR_STRIDE, (name, place)
+
+
 def test_python_operators_refuse_cpu_tensors():
     from ebr_b200 import token_ops as tk
 
