@@ -413,6 +413,38 @@ def test_expert_second_order_matches_plain_autograd():
         assert float((a.double() - b).abs().max()) <= 2e-5 * float(b.abs().max())
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("capacity", [None, 9])
+def test_expert_second_order_of_each_type_with_dropped_slots(dtype, capacity):
+    """The derivatives of <d rows, a> + <d w, b> + <d x, d>, where d rows, d w and d x are the gradients of the combine and
+    the dispatch: products and sums over slots again, one rounding each and one for a sum of two."""
+    from ebr_b200.token_ops import expert_combine, expert_dispatch, expert_route
+
+    t, k, e, c = 40, 3, 7, 72
+    r = expert_route(randint(-1, e, (t, k), seed=3), e, capacity)
+    assert bool((r.row_of < 0).any())
+    live = (r.row_of >= 0).unsqueeze(-1)
+    for wtype in {torch.float32, dtype}:
+        rows, gy, a = rand(r.rows, c, seed=1, dtype=dtype), rand(t, c, seed=2, dtype=dtype), rand(r.rows, c, seed=4, dtype=dtype)
+        w, b = rand(t, k, seed=5, dtype=wtype), rand(t, k, seed=6, dtype=wtype)
+        rows, gy, w = (v.requires_grad_(True) for v in (rows, gy, w))
+        grows, gw = torch.autograd.grad(expert_combine(rows, r, w), [rows, w], gy, create_graph=True)
+        drows, dw, dgy = torch.autograd.grad([grows, gw], [rows, w, gy], [a, b])
+        assert drows.dtype == dgy.dtype == dtype and dw.dtype == wtype
+        slack = 2 * E + U[dtype]
+        ref = plain_dispatch(gy.detach(), r, b)
+        assert_within(drows, ref, slack * ref.abs() + TINY[dtype])
+        terms = a.double()[r.row_of.clamp(min=0).long()] * gy.detach().double().unsqueeze(1) * live
+        assert_within(dw, terms.sum(-1), (c + 2) * E * terms.abs().sum(-1) + U[wtype] * terms.sum(-1).abs() + TINY[wtype])
+        (one, m1), (two, m2) = plain_combine(a, r, w.detach()), plain_combine(rows.detach(), r, b)
+        bound = (k + 2) * E * (m1 + m2) + U[dtype] * (one.abs() + two.abs() + (1 + U[dtype]) * (one + two).abs()) * 1.01
+        assert_within(dgy, one + two, bound + 3 * TINY[dtype])
+        x, gs = rand(t, c, seed=7, dtype=dtype).requires_grad_(True), rand(r.rows, c, seed=8, dtype=dtype).requires_grad_(True)
+        d = rand(t, c, seed=9, dtype=dtype)
+        (gx,) = torch.autograd.grad(expert_dispatch(x, r), x, gs, create_graph=True)
+        assert torch.equal(torch.autograd.grad(gx, gs, d)[0].double(), plain_dispatch(d, r))
+
+
 def test_expert_gradients_by_differences():
     """The combine is bilinear: central differences are exact up to rounding, whatever the step."""
     from ebr_b200.token_ops import expert_combine, expert_route
@@ -587,6 +619,39 @@ def test_distillation_against_float64(n, v, k, dtype):
     logits = rand(n, v, seed=1) * 3
     logits.scatter_add_(1, ids.clamp(min=0), rand(n, k, seed=2).abs())
     check_distill(logits.to(dtype), ids, (rand(n, k, seed=3) * 2 + 3).to(dtype), 1.7)
+
+
+@pytest.mark.parametrize("n,v,dtype", [
+    (2700, 17000, torch.bfloat16),  # rings of 8 KB chunks, 888 CTAs: three and four rows each
+    (900, 70001, torch.bfloat16),   # rings of 24 KB chunks, 296 CTAs: three and four rows each
+    (200, 131073, torch.float32),   # clusters of two, 148 of them: a second row for some
+])  # fmt: skip
+def test_distillation_of_several_rows_to_a_ring(n, v, dtype):
+    """Rows that do not count among those that do: the first of a CTA, several in a row, the last; and the others' values."""
+    ids, top = randint(-1, v, (n, 6), seed=1), rand(n, 6, seed=2)
+    logits = (rand(n, v, seed=3) * 2).to(dtype)
+    weight = rand(n, seed=4).abs() + 0.25
+    ids[[0, 1, 2, 148, 149, 297, n - 1] if n > 297 else [0, 1, 2, 148, 149, n - 1]] = -1
+    weight[[1, 3, 4, 150, 151, n // 2, n - 2]] = 0
+    logits[[0, 3, 150]] = math.nan
+    check_distill(logits, ids, top, 1.3, weight)
+
+
+def test_distillation_of_long_rows_repeats_bit_for_bit_on_another_stream():
+    from ebr_b200.token_ops import topk_distill_loss
+
+    for n, v in ((1000, 33000), (400, 70001)):
+        x = rand(n, v, seed=1, dtype=torch.bfloat16).requires_grad_(True)
+        ids, top = randint(-1, v, (n, 12), seed=2), rand(n, 12, seed=3)
+        a = topk_distill_loss(x, ids, top)
+        (ga,) = torch.autograd.grad(a, x)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            b = topk_distill_loss(x, ids, top)
+            (gb,) = torch.autograd.grad(b, x)
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(a, b) and torch.equal(ga, gb)
 
 
 @pytest.mark.parametrize("v", [10, 700, 20000, 70000])
