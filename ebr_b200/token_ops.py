@@ -49,19 +49,9 @@ def _require(t: Tensor, what: str, name: str, types: dict, device: Optional[torc
 
 def _has_tangent(*tensors: Optional[Tensor]) -> bool:
     """Whether one of them carries a forward-mode tangent, which no kernel here propagates: such a call goes through its
-    autograd Function, which refuses it. A direct call would drop it, and a dropped tangent counts as zero."""
-    if forward_ad._current_level < 0:
-        return False
+    autograd Function, which refuses it. A direct call would drop it, and a dropped tangent counts as zero. Asked for only
+    inside a forward-mode level (``forward_ad._current_level >= 0``): elsewhere there are none, and a call is short."""
     return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
-
-
-def _recorded(*tensors: Optional[Tensor]) -> bool:
-    """Whether a call goes through its autograd Function."""
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                return True
-    return _has_tangent(*tensors)
 
 
 def _fine(t: Tensor, types: dict) -> bool:
@@ -155,7 +145,7 @@ class _Embed(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g: Tensor):
         (tokens,) = ctx.saved_tensors
-        if torch.is_grad_enabled() or _has_tangent(g):
+        if torch.is_grad_enabled() or forward_ad._current_level >= 0 and _has_tangent(g):
             return _EmbedGrad.apply(g, tokens, ctx.scale, ctx.rows, ctx.dtype), None, None, None
         return _lookup_grad(tokens, g, ctx.scale, ctx.rows, ctx.dtype), None, None, None
 
@@ -190,7 +180,7 @@ def scaled_embedding(tokens: Tensor, weight: Tensor, scale: float = 1.0, dtype: 
     if dtype not in _DTYPES:
         raise TypeError(f"scaled_embedding: unsupported output dtype {dtype}")
     tokens = tokens if tokens.is_contiguous() else tokens.contiguous()
-    if _recorded(weight):
+    if torch.is_grad_enabled() and weight.requires_grad or forward_ad._current_level >= 0 and _has_tangent(weight):
         return _Embed.apply(weight, tokens, float(scale), dtype)
     return _lookup(tokens, weight, float(scale), dtype)
 
@@ -299,7 +289,8 @@ class _Dispatch(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g: Tensor):
         route = ctx.route
-        if not (ctx.weighted or torch.is_grad_enabled() or _has_tangent(g)):
+        direct = not (torch.is_grad_enabled() or forward_ad._current_level >= 0 and _has_tangent(g))
+        if direct and not ctx.weighted:
             return _combine(g, route, None), None, None
         x, weights = ctx.saved_tensors if ctx.weighted else (None, None)
         gx = _Combine.apply(g, weights, route) if ctx.needs_input_grad[0] else None
@@ -323,7 +314,8 @@ class _Combine(torch.autograd.Function):
         route = ctx.route
         rows, weights = ctx.saved_tensors if ctx.weighted else (None, None)
         need_rows, need_weights = ctx.needs_input_grad[:2]
-        if need_rows and need_weights and ctx.weighted and not torch.is_grad_enabled() and not _has_tangent(g):
+        direct = not (torch.is_grad_enabled() or forward_ad._current_level >= 0 and _has_tangent(g))
+        if direct and need_rows and need_weights and ctx.weighted:
             grows, gw = _scatter(_as(g, rows.dtype), route, weights, rows, True)  # both in one pass over g and the rows
             return grows, _as(gw, weights.dtype), None
         grows = _Dispatch.apply(g, weights, route) if need_rows else None
@@ -358,7 +350,7 @@ def expert_dispatch(x: Tensor, route: ExpertRoute) -> Tensor:
         raise ValueError(
             f"expert_dispatch: x must be [*{tuple(route.row_of.shape[:-1])}, C] for this route, got {tuple(x.shape)}"
         )
-    if _recorded(x):
+    if torch.is_grad_enabled() and x.requires_grad or forward_ad._current_level >= 0 and _has_tangent(x):
         return _Dispatch.apply(x, None, route)
     return _scatter(x, route, None, None, True)[0]
 
@@ -379,7 +371,8 @@ def expert_combine(rows: Tensor, route: ExpertRoute, weights: Optional[Tensor] =
             raise ValueError(
                 f"expert_combine: weights must be {tuple(route.row_of.shape)} for this route, got {tuple(weights.shape)}"
             )
-    if _recorded(rows, weights):
+    if (torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad))
+            or forward_ad._current_level >= 0 and _has_tangent(rows, weights)):  # fmt: skip
         return _Combine.apply(rows, weights, route)
     return _combine(rows, route, weights)
 
@@ -465,7 +458,7 @@ class _TopkDistill(torch.autograd.Function):
 
     @staticmethod
     def _backward(ctx, g: Tensor):
-        if _has_tangent(g):
+        if forward_ad._current_level >= 0 and _has_tangent(g):
             raise NotImplementedError("topk_distill_loss has no forward-mode derivative")
         view, ids, top, row_weight, stats = ctx.saved_tensors
         made, ctx.made = ctx.made, None
@@ -493,14 +486,15 @@ def topk_distill_loss(logits: Tensor, teacher_ids: Tensor, teacher_logits: Tenso
         _require(logits, what, "logits", _DTYPES)
         _require(teacher_ids, what, "teacher_ids", _IDS, logits.device)
         _require(teacher_logits, what, "teacher_logits", _DTYPES, logits.device)
-    if logits.dim() < 1 or teacher_ids.dim() < 1 or teacher_ids.shape[:-1] != logits.shape[:-1] or not logits.shape[-1]:
+    shape, entries = logits.shape, teacher_ids.shape
+    if not shape or not entries or entries[:-1] != shape[:-1] or not shape[-1]:
         raise ValueError(f"{what}: logits [..., V] and teacher_ids [..., K] must have the same rows, got "
-                         f"{tuple(logits.shape)} and {tuple(teacher_ids.shape)}")  # fmt: skip
-    if teacher_logits.shape != teacher_ids.shape or not 1 <= teacher_ids.shape[-1] <= 1024:
+                         f"{tuple(shape)} and {tuple(entries)}")  # fmt: skip
+    if teacher_logits.shape != entries or not 1 <= entries[-1] <= 1024:
         raise ValueError(f"{what}: teacher_logits must be shaped as teacher_ids with 1 to 1024 entries a row, got "
-                         f"{tuple(teacher_logits.shape)} and {tuple(teacher_ids.shape)}")  # fmt: skip
-    if logits.shape[-1] > 1 << 19:
-        raise ValueError(f"{what}: a vocabulary of at most {1 << 19}, got {logits.shape[-1]}")
+                         f"{tuple(teacher_logits.shape)} and {tuple(entries)}")  # fmt: skip
+    if shape[-1] > 1 << 19:
+        raise ValueError(f"{what}: a vocabulary of at most {1 << 19}, got {shape[-1]}")
     if not 2.0**-126 <= temperature <= 1e30:
         raise ValueError(f"{what}: the temperature must be between 1.2e-38 and 1e30, got {temperature}")
     if reduction not in ("none", "sum", "mean"):
@@ -509,15 +503,16 @@ def topk_distill_loss(logits: Tensor, teacher_ids: Tensor, teacher_logits: Tenso
         raise ValueError(f"{what}: the teacher and the row weights are constants; detach them")
     if row_weight is not None:
         _require(row_weight, what, "row_weight", _DTYPES, logits.device)
-        if row_weight.shape != logits.shape[:-1]:
-            raise ValueError(f"{what}: row_weight must be {tuple(logits.shape[:-1])}, got {tuple(row_weight.shape)}")
+        if row_weight.shape != shape[:-1]:
+            raise ValueError(f"{what}: row_weight must be {tuple(shape[:-1])}, got {tuple(row_weight.shape)}")
         row_weight = row_weight.to(torch.float32).contiguous()
     ids = teacher_ids if teacher_ids.is_contiguous() else teacher_ids.contiguous()
     top = teacher_logits if teacher_logits.is_contiguous() else teacher_logits.contiguous()
-    rows = ids.numel() // ids.shape[-1]
+    rows = ids.numel() // entries[-1]
     factor = 1.0 / rows if reduction == "mean" and rows else 1.0
     reduced = reduction != "none"
-    if _recorded(logits, top, row_weight):
+    if (torch.is_grad_enabled() and logits.requires_grad
+            or forward_ad._current_level >= 0 and _has_tangent(logits, top, row_weight)):  # fmt: skip
         return _TopkDistill.apply(logits, ids, top, float(temperature), row_weight, factor, reduced)
     losses, total, _, _ = _distill(*_row_view(logits), ids, top, float(temperature), row_weight, factor, reduced, False)
     return total if reduced else losses
