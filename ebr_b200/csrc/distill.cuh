@@ -8,11 +8,14 @@
 // loss is tau times their sum: neither 1 / tau nor tau^2 is formed, which leave float32 at temperatures (and at masked
 // logits) whose losses do not.
 //
-// Measured, bfloat16, 64 entries, loss and gradient in one pass: 4,096 rows of 131,072 take 444 us (4.8 TB/s of
+// Measured, bfloat16, 64 entries, loss and gradient in one pass: 4,096 rows of 131,072 take 436 to 444 us (4.8 TB/s of
 // logits and gradient; the loss alone 202, 5.3 TB/s; the gradient alone 348, 6.2 TB/s), 16,384 of 32,768 504 us,
 // 65,536 of 8,192 515 us, 131,072 of 4,096 (16 entries) 394 us (5.5 TB/s). The one-pass kernel is bound by latency,
-// issue and the exponential unit together (58 and 54 % busy with sixteen warps on an SM at 463 us); the rings leave
-// room for 24.
+// issue and the exponential unit together (61 and 58 % busy with the 24 warps that the rings leave room for on an SM).
+// The warp kernel misses L2 at its second reading of rows of 8 to 32 KB: at 8,192 rows of 16,384 it reads 594 MB from
+// HBM for 268 MB of logits. Rows whose gradient starts at another place of a 16-byte word (a view of rows that are more
+// than 256 elements longer, by a number that is no multiple of 16 bytes) are stored element by element: 8,388 rows of
+// 32,001 take 868 us so, 269 where the places agree.
 #pragma once
 
 #include "../../include/ebr_tokens.h"

@@ -8,10 +8,13 @@
 // crosses chunks leaves one float32 partial sum per chunk, which a second kernel adds in chunk order. A table of ten
 // rows under 62,208 tokens (runs of thousands) and one of 131,072 rows (runs of one or two) take the same path.
 //
-// Measured: the lookup of 16,384 bfloat16 tokens of 2,048 columns 16.5 us (8.1 TB/s of its rows and output, some of
-// it from L2), of 62,208 board tokens of 512 columns from a float32 table 17 us (3.7 TB/s: the table's rows come from
-// L1 as 32 bytes a lane); the gradients of the same 111 us (5.5 TB/s; 74 of it zero the table, beside the sort) and
-// 31 us (chunks 17, the join 8, the sort 7: the latency of four short kernels).
+// Measured, replayed from a CUDA graph (warm: one after another; cold: behind a flush of L2): the lookup of 16,384
+// bfloat16 tokens of 2,048 columns 16.5 us warm (8.1 TB/s of its rows and output, some of it from L2), of 62,208 board
+// tokens of 512 columns from a float32 table 16.4 us warm and 20.5 cold (3.9 and 3.1 TB/s: the latency of a single
+// wave of 3,900 warps with four rows in flight each; issue slots 41 %, resident warps 38 %); the gradients of the same
+// 111 us warm (5.5 TB/s; 74 of it zero the table, beside the sort) and 27 us warm, 39 to 41 cold (the latency of four
+// short kernels: two of the sort, chunks, join). Rows of an odd number of 16-bit elements go two bytes a lane: 30,000
+// tokens of 1,001 bfloat16 of a table of 50,000 take 31 us (lookup) and 86 (gradient) warm, of 1,000 columns 21 and 53.
 #pragma once
 
 #include <type_traits>

@@ -294,8 +294,9 @@ int check_embedding(int id_type, int64_t n, int64_t V, int64_t C, int64_t stride
   return EBR_OK;
 }
 
-// Rows of a chunk of the gradient, 8 to 256: some 3,000 warps' worth of chunks (62,208 board tokens of 512 columns:
-// the whole gradient takes 35 us with 64 rows, 42 with 32, which leave twice the partial sums to join).
+// Rows of a chunk of the gradient, 8 to 256: up to 3,500 warps' worth of chunks. 62,208 board tokens of 512 columns:
+// the whole gradient takes 26.6 us warm and 39 cold with 64 rows, 32.8 and 47 with 32, which leave twice the partial
+// sums to join, 28.7 and 45 with 128, which leave half the warps.
 int64_t grad_chunk_rows(int64_t n, int64_t C) {
   const int64_t blocks = (C + 255) / 256;
   int64_t r = 8;
@@ -409,8 +410,8 @@ int launch_distill(int device, const ebr::distill::Args& a, cudaStream_t st) {
   while (slices < ebr::distill::kMaxSlices && a.N * slices < 2 * sm_count(device) && (total + slices - 1) / slices > 256)
     slices *= 2;
   const int granules = static_cast<int>((total + slices - 1) / slices);
-  // Rows above 128 KB: rings of four 24 KB chunks, two on an SM, 24 warps; shorter rows want more rows in flight:
-  // rings of four 8 KB chunks, six on an SM. bfloat16 at 2.1 GB: V = 131,072 takes 0.44 ms with the first, 0.55 with
+  // Slices above 128 KB (a row's, where it is not split): rings of four 24 KB chunks, two on an SM, 24 warps; shorter
+  // ones want more rows in flight: rings of four 8 KB chunks, six on an SM. bfloat16 at 2.1 GB: V = 131,072 takes 0.44 ms with the first, 0.55 with
   // the second; V = 32,768 takes 0.56 and 0.50.
   const int rc = granules > 8192 ? launch_distill_row<T, 12, 4>(device, a, slices, granules, 4, 2, st)
                                  : launch_distill_row<T, 4, 4>(device, a, slices, granules, 4, 6, st);

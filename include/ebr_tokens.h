@@ -51,7 +51,7 @@ size_t ebr_expert_route_scratch_bytes(int64_t T, int64_t K, int64_t E);
  * zeros; x [T, C] (row stride x_stride, unit column stride), rows_out [rows, C] contiguous. With rows_in [rows, C] and
  * dots [T, K] (both or neither), also dots[t, k] = <x[t, :], rows_in[row_of[t, k], :]> (0 for a dropped slot): with x
  * the gradient of ebr_expert_combine's output, the gradients of its rows and weights. rows_out may be NULL when dots is
- * not. weights and dots have type weight_dtype: EBR_FLOAT32 or dtype. */
+ * not. weights and dots have type weight_dtype: EBR_FLOAT32 or dtype. Every row_of value is in [-1, rows). */
 int ebr_expert_scatter(int dtype, int weight_dtype, int64_t T, int64_t K, int64_t C, int64_t rows, const void* x,
                        int64_t x_stride, const int32_t* row_of, const int32_t* slot_of, const void* weights,
                        const void* rows_in, void* rows_out, void* dots, void* stream);

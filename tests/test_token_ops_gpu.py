@@ -983,6 +983,25 @@ def test_forward_mode_is_refused():
         assert torch.equal(scaled_embedding(tokens, w), w[tokens])  # tensors without a tangent are as ever
 
 
+def test_compiled_callers_get_the_same_results():
+    """torch.compile breaks its graph at the operators and runs them as they are."""
+    from ebr_b200.token_ops import expert_combine, expert_dispatch, expert_route, scaled_embedding, topk_distill_loss
+
+    def f(tokens, w, experts, weights, ids, top):
+        h = scaled_embedding(tokens, w, 2.0).tanh()
+        r = expert_route(experts, 4, 12)
+        return topk_distill_loss(expert_combine(expert_dispatch(h, r) * 2, r, weights) + h, ids, top, 1.5)
+
+    args = [randint(0, 6, (20,), seed=1), rand(6, 32, seed=2).requires_grad_(True), randint(0, 4, (20, 2), seed=3),
+            rand(20, 2, seed=4).requires_grad_(True), randint(-1, 32, (20, 3), seed=5), rand(20, 3, seed=6)]  # fmt: skip
+    results = []
+    for call in (f, torch.compile(f, backend="eager")):
+        loss = call(*args)
+        results.append((loss, *torch.autograd.grad(loss, [args[1], args[3]])))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+
+
 def test_expert_network_matches_plain_experts_to_second_order():
     """E, dE/dv and d<dE/dv, u>/d(v, weights) of the float32 network against the same network with a plain sparse MLP:
     1e-4 of the norms, the bar of the dense float32 network's fixtures."""
