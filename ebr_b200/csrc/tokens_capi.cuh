@@ -411,8 +411,8 @@ int launch_distill(int device, const ebr::distill::Args& a, cudaStream_t st) {
     slices *= 2;
   const int granules = static_cast<int>((total + slices - 1) / slices);
   // Slices above 128 KB (a row's, where it is not split): rings of four 24 KB chunks, two on an SM, 24 warps; shorter
-  // ones want more rows in flight: rings of four 8 KB chunks, six on an SM. bfloat16 at 2.1 GB: V = 131,072 takes 0.44 ms with the first, 0.55 with
-  // the second; V = 32,768 takes 0.56 and 0.50.
+  // ones want more rows in flight: rings of four 8 KB chunks, six on an SM. bfloat16 at 2.1 GB: V = 131,072 takes
+  // 0.44 ms with the first, 0.55 with the second; V = 32,768 takes 0.56 and 0.50.
   const int rc = granules > 8192 ? launch_distill_row<T, 12, 4>(device, a, slices, granules, 4, 2, st)
                                  : launch_distill_row<T, 4, 4>(device, a, slices, granules, 4, 6, st);
   return rc != EBR_OK ? rc : launch_distill_entries<T, true>(a, st);

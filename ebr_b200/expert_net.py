@@ -48,7 +48,8 @@ class ExpertShape(NetShape):
 class _RouterScores(torch.autograd.Function):
     """h W^T in float32, h and W as they are: scores rounded to 16 bits would leave near ties between experts to the
     rounding. The backward is a 16-bit product's, with the scores' gradient rounded as any activation's, and is
-    differentiable. (Casting h and W to float32 instead took a training step of 768 boards from 24 to 26 ms.)"""
+    differentiable. It makes both gradients whichever is asked for: 0.04 ms of a microstep of 768 boards, which takes 5.6.
+    (Casting h and W to float32 instead took a training step of 768 boards from 24 to 26 ms.)"""
 
     @staticmethod
     def forward(ctx, h: Tensor, w: Tensor) -> Tensor:

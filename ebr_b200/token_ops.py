@@ -476,9 +476,9 @@ def topk_distill_loss(logits: Tensor, teacher_ids: Tensor, teacher_logits: Tenso
     ``logits`` [..., V] in float32, float16 or bfloat16; ``teacher_ids`` [..., K] int32 or int64, an id outside ``[0, V)``
     being no entry (a shorter list, a masked row); ``teacher_logits`` [..., K]; ``row_weight`` [...] multiplies the rows'
     losses. A row without entries, with entries of -inf alone, or of weight 0, has loss 0 and gradient 0 whatever its logits
-    hold. ``reduction``: ``"none"`` (the rows' losses, float32), ``"sum"`` or ``"mean"`` (the sum over the number of rows). Differentiable once,
-    in ``logits``; the teacher and the weights are constants. A reduced loss keeps a gradient of the logits' size from the
-    forward to the backward pass. Logits whose rows do not lie one stride apart are copied, once: leave positions out by
+    hold. ``reduction``: ``"none"`` (the rows' losses, float32), ``"sum"`` or ``"mean"`` (the sum over the number of rows).
+    Differentiable once, in ``logits``; the teacher and the weights are constants. A reduced loss keeps a gradient of the
+    logits' size from the forward to the backward pass. Logits whose rows do not lie one stride apart are copied, once: leave positions out by
     ``row_weight`` or padding ids rather than by a slice such as ``logits[:, :-1]``."""
     what = "topk_distill_loss"
     if not (_fine(logits, _DTYPES) and _fine(teacher_ids, _IDS) and _fine(teacher_logits, _DTYPES)
